@@ -69,12 +69,22 @@ class AmberGraphDesc(C.Structure):
                                          "reserved")] + [("edge_capacity", C.c_int64), ("edge_offset", C.c_int64)]
 
 
+DTYPE = {"float32": 0, "bfloat16": 1, "float16": 2}  # AMBER_DTYPE_*
+ACT_NONE = -1
+
+
+class AmberTailDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("activation", C.c_int32), ("normalize", C.c_int32),
+                ("p", C.c_double), ("eps", C.c_double), ("sequence", C.c_int64)]
+
+
 _P = C.c_void_p
 _I64 = C.c_int64
 _I32 = C.c_int32
 _SZ = C.c_size_t
 _DESC = C.POINTER(AmberMpnDesc)
 _GLUE = C.POINTER(AmberGlueDesc)
+_TAIL = C.POINTER(AmberTailDesc)
 _F64 = C.c_double
 
 # name -> (restype, argtypes): every symbol include/amber_mpn.h declares
@@ -113,6 +123,11 @@ SIGNATURES = {
     "amber_mpn_project_elements_to_vertices": (C.c_int, [_P, _I32, _I64, _I64, _P, _P, _P, _P, _P, _SZ, _P]),
     "amber_mpn_estimate_workspace_bytes": (_SZ, [_I64, _I64]),
     "amber_mpn_estimate_num_elements": (C.c_int, [_P, _I32, _I64, _I64, _P, _P, _I32, _I32, _P, _I64, _P, _F64, _P, _P, _SZ, _P]),
+    "amber_mpn_generator_take": (C.c_int, [_P, _I64, _P, _P]),
+    "amber_mpn_keep_mask": (C.c_int, [_P, _I64, _F64, _I64, _P, _P]),
+    "amber_mpn_tail_forward": (C.c_int, [_TAIL, _I64, _I64, _P, _I64, _P, _P, _P, _P, _P, _P]),
+    "amber_mpn_tail_backward_workspace_bytes": (_SZ, [_TAIL, _I64, _I64]),
+    "amber_mpn_tail_backward": (C.c_int, [_TAIL, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "amber_mpn_predict_workspace_bytes": (_SZ, [_DESC, _I64, _I64]),
     "amber_mpn_predict": (C.c_int, [_DESC, _GLUE, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                     _P, _SZ, _P]),

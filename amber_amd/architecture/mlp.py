@@ -3,12 +3,14 @@
 Per layer: Linear -> activation [-> LayerNorm | BatchNorm1d] [-> Dropout], with the same ModuleList indices as the
 reference so `decoder_mlp.mlp_layers.{i}.*` checkpoint keys load.  Runs fused in the last node kernel (K10).
 """
-from typing import List, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 from torch import nn as nn
 from torch.nn.utils import spectral_norm as apply_spectral_norm
 from torch.nn.utils.spectral_norm import SpectralNorm
+
+from amber_amd.norm_dropout import CounterGenerator, activate_norm_dropout, dropout
 
 _ACTIVATIONS = {"relu": nn.ReLU, "leakyrelu": nn.LeakyReLU, "elu": nn.ELU, "swish": nn.SiLU, "silu": nn.SiLU,
                 "mish": nn.Mish, "gelu": nn.GELU, "tanh": nn.Tanh}
@@ -109,6 +111,35 @@ class MLP(nn.Module):
             if i < len(mods) and isinstance(mods[i], nn.Dropout):
                 i += 1  # identity in eval mode
         return pieces, sources
+
+    def run_layers(self, tensor: torch.Tensor, generator: Optional[CounterGenerator] = None) -> torch.Tensor:
+        """The layers one by one, as the reference's MLP.forward (mlp.py:128-129).  With a generator everything after a
+        Linear is one pass (activation, LayerNorm, dropout from the counter-based generator); BatchNorm stays torch's."""
+        if generator is None:
+            for layer in self.mlp_layers:
+                tensor = layer(tensor)
+            return tensor
+        mods = list(self.mlp_layers)
+        drops = sum(isinstance(m, nn.Dropout) and m.training and m.p > 0 for m in mods)
+        state = generator.take(drops) if drops else None
+        sequence = 0
+        for i, lin in enumerate(mods):
+            if not isinstance(lin, nn.Linear):
+                continue
+            tail = mods[i + 2:next((j for j in range(i + 1, len(mods)) if isinstance(mods[j], nn.Linear)), len(mods))]
+            ln = next((m for m in tail if isinstance(m, nn.LayerNorm)), None)
+            bn = next((m for m in tail if isinstance(m, nn.BatchNorm1d)), None)
+            drop = next((m for m in tail if isinstance(m, nn.Dropout) and m.training and m.p > 0), None)
+            p = drop.p if drop is not None else 0.0
+            tensor = lin(tensor)
+            if bn is not None:
+                tensor = dropout(bn(mods[i + 1](tensor)), p, state, sequence=sequence)
+            else:
+                tensor = activate_norm_dropout(tensor, self.activation_function, ln.weight if ln is not None else None,
+                                               ln.bias if ln is not None else None, normalize=ln is not None,
+                                               eps=ln.eps if ln is not None else 0.0, p=p, state=state, sequence=sequence)
+            sequence += drop is not None
+        return tensor
 
     def forward(self, tensor: torch.Tensor) -> torch.Tensor:
         raise RuntimeError("amber_amd.MLP holds parameters only; the decoder runs fused inside SupervisedMPN.forward (HIP).")

@@ -28,7 +28,8 @@ class SupervisedMPN(nn.Module):
     def __init__(self, architecture_config, example_graph):
         """architecture_config: `.latent_dimension`, `.decoder` and `.get(...)` for create_graph_copy,
         assert_graph_shapes, stack, embedding, edge_dropout (an omegaconf DictConfig in the reference; any object
-        with attribute access and `.get` works).  example_graph fixes the raw feature widths."""
+        with attribute access and `.get` works), and dropout_generator / dropout_seed (see get_mpn).  example_graph
+        fixes the raw feature widths."""
         super().__init__()
         self._node_type = "node"
         latent_dimension = architecture_config.latent_dimension
@@ -105,13 +106,13 @@ class SupervisedMPN(nn.Module):
         return has_bn and torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters())
 
     def _forward_module_decoder(self, observations) -> torch.Tensor:
-        """supervised_mpn.py:48-54 with the stack on the HIP path (autograd through amber_mpn_backward for the latents)."""
+        """supervised_mpn.py:48-54 with the stack on the HIP path (autograd through amber_mpn_backward for the latents) and, with
+        `dropout_generator: counter`, what follows each Linear as one HIP pass."""
         node_features, _, _ = self.mpn(observations)
         node_features = node_features.get(self._node_type)
         if hasattr(observations, "mask_output"):
             node_features = node_features[observations.mask_output]
-        for layer in self.decoder_mlp.mlp_layers:
-            node_features = layer(node_features)
+        node_features = self.decoder_mlp.run_layers(node_features, self.mpn.dropout_generator)
         return self.readout(node_features)
 
     def _check_train_mode_decoder(self):

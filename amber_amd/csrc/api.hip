@@ -1453,6 +1453,135 @@ int amber_mpn_inverse_transform(int32_t transform, const float* in, const float*
   return AMBER_OK;
 }
 
+// ---- activation -> LayerNorm -> dropout --------------------------------------------------------------------------
+// p as the kernels take it: an element is dropped iff its 32-bit word is <= last; drop = 0: no element is
+static void set_dropout(double p, TailArgs& a) {
+  const double t = p * 4294967296.0;  // exact: a power of two
+  a.drop = t >= 1.0;
+  a.last_dropped = t >= 4294967296.0 ? 0xFFFFFFFFu : a.drop ? static_cast<uint32_t>(t) - 1u : 0u;
+  a.scale = p < 1.0 ? static_cast<float>(1.0 / (1.0 - p)) : 0.f;
+}
+static int make_tail_args(const AmberTailDesc* d, int64_t rows, int64_t width, const int64_t* state, bool need_state, TailArgs& a) {
+  if (!d) return fail(AMBER_ERR_INVALID_ARGUMENT, "desc is NULL");
+  if (d->dtype < AMBER_DTYPE_F32 || d->dtype > AMBER_DTYPE_F16) return fail(AMBER_ERR_UNSUPPORTED, "dtype id %d", d->dtype);
+  if (d->weight_dtype != AMBER_DTYPE_F32 && d->weight_dtype != d->dtype)
+    return fail(AMBER_ERR_UNSUPPORTED, "weight_dtype id %d with dtype id %d", d->weight_dtype, d->dtype);
+  if (d->activation < AMBER_ACT_NONE || d->activation > AMBER_ACT_GELU)
+    return fail(AMBER_ERR_UNSUPPORTED, "activation id %d", d->activation);
+  if (!(d->p >= 0.0 && d->p <= 1.0)) return fail(AMBER_ERR_INVALID_ARGUMENT, "dropout probability has to be between 0 and 1");
+  if (!(d->eps >= 0.0 && d->eps <= 3.0e38)) return fail(AMBER_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
+  if (d->sequence < 0) return fail(AMBER_ERR_INVALID_ARGUMENT, "negative sequence");
+  if (rows < 0 || width < 0) return fail(AMBER_ERR_INVALID_ARGUMENT, "negative size");
+  if (width >= (1ll << 31) || (width > 0 && rows > (1ll << 50) / width))
+    return fail(AMBER_ERR_INVALID_ARGUMENT, "rows / width out of range");
+  if (d->normalize && width == 0) return fail(AMBER_ERR_INVALID_ARGUMENT, "LayerNorm over no features");
+  a = TailArgs{};
+  a.rows = rows;
+  a.width = width;
+  a.dtype = d->dtype;
+  a.weight_dtype = d->weight_dtype;
+  a.act = d->activation;
+  a.eps = static_cast<float>(d->eps);
+  a.sequence = d->sequence;
+  a.state = state;
+  set_dropout(d->p, a);
+  if (need_state && a.drop && rows * width > 0 && !state) return fail(AMBER_ERR_INVALID_ARGUMENT, "state is NULL");
+  return AMBER_OK;
+}
+
+int amber_mpn_generator_take(int64_t* state, int64_t count, int64_t* taken, void* stream) {
+  if (!state || !taken) return fail(AMBER_ERR_INVALID_ARGUMENT, "state / taken is NULL");
+  if (count < 0) return fail(AMBER_ERR_INVALID_ARGUMENT, "negative count");
+  (void)hipGetLastError();
+  HIP_TRY(launch_generator_take(state, count, taken, static_cast<hipStream_t>(stream)), "generator take");
+  return AMBER_OK;
+}
+
+int amber_mpn_keep_mask(const int64_t* state, int64_t sequence, double p, int64_t n, uint8_t* out, void* stream) {
+  AmberTailDesc d{};
+  d.activation = AMBER_ACT_NONE;
+  d.p = p;
+  d.sequence = sequence;
+  TailArgs a;
+  int rc = make_tail_args(&d, n, 1, state, true, a);
+  if (rc) return rc;
+  if (n == 0) return AMBER_OK;
+  if (!out) return fail(AMBER_ERR_INVALID_ARGUMENT, "out is NULL");
+  (void)hipGetLastError();
+  HIP_TRY(launch_keep_mask(a, out, static_cast<hipStream_t>(stream)), "keep_mask");
+  return AMBER_OK;
+}
+
+int amber_mpn_tail_forward(const AmberTailDesc* desc, int64_t rows, int64_t width, const void* x, int64_t x_stride,
+                           const void* weight, const void* bias, const int64_t* state, void* y, float* stats, void* stream) {
+  TailArgs a;
+  int rc = make_tail_args(desc, rows, width, state, true, a);
+  if (rc) return rc;
+  if (rows == 0 || width == 0) return AMBER_OK;
+  if (!x || !y) return fail(AMBER_ERR_INVALID_ARGUMENT, "x / y is NULL");
+  if (x_stride < 0 || x_stride > (1ll << 50) / rows) return fail(AMBER_ERR_INVALID_ARGUMENT, "x_stride out of range");
+  if (!desc->normalize && (weight || bias)) return fail(AMBER_ERR_INVALID_ARGUMENT, "weight / bias without normalize");
+  if (!desc->normalize && rows > 1 && x_stride != width) return fail(AMBER_ERR_UNSUPPORTED, "strided rows without normalize");
+  a.x = x;
+  a.ldx = x_stride;
+  a.weight = weight;
+  a.bias = bias;
+  a.y = y;
+  a.stats = stats;
+  (void)hipGetLastError();
+  HIP_TRY(launch_tail_forward(a, desc->normalize != 0, static_cast<hipStream_t>(stream)), "tail forward");
+  return AMBER_OK;
+}
+
+size_t amber_mpn_tail_backward_workspace_bytes(const AmberTailDesc* desc, int64_t rows, int64_t width) {
+  TailArgs a;
+  if (make_tail_args(desc, rows, width, nullptr, false, a)) return 0;
+  if (!desc->normalize || rows == 0) return 256;
+  return align256(sizeof(float) * 2 * static_cast<size_t>(width) * static_cast<size_t>(tail_partial_blocks(a))) + 256;
+}
+
+int amber_mpn_tail_backward(const AmberTailDesc* desc, int64_t rows, int64_t width, const void* x, int64_t x_stride,
+                            const void* grad_y, int64_t g_stride, const void* weight, const float* stats, const int64_t* state,
+                            void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+  TailArgs a;
+  int rc = make_tail_args(desc, rows, width, state, true, a);
+  if (rc) return rc;
+  const bool norm = desc->normalize != 0;
+  if (!norm && (weight || grad_weight || grad_bias)) return fail(AMBER_ERR_INVALID_ARGUMENT, "weight / bias without normalize");
+  if (width == 0 || (rows == 0 && !grad_weight && !grad_bias)) return AMBER_OK;
+  if (rows > 0) {
+    if (!grad_y) return fail(AMBER_ERR_INVALID_ARGUMENT, "grad_y is NULL");
+    if ((norm || a.act != AMBER_ACT_NONE) && !x) return fail(AMBER_ERR_INVALID_ARGUMENT, "x is NULL");
+    if (norm && !stats) return fail(AMBER_ERR_INVALID_ARGUMENT, "stats is NULL");
+    if (x_stride < 0 || x_stride > (1ll << 50) / rows || g_stride < 0 || g_stride > (1ll << 50) / rows)
+      return fail(AMBER_ERR_INVALID_ARGUMENT, "row stride out of range");
+    if (!norm && rows > 1 && ((x && x_stride != width) || g_stride != width))
+      return fail(AMBER_ERR_UNSUPPORTED, "strided rows without normalize");
+  }
+  if (!norm && !grad_x) return AMBER_OK;
+  a.x = x;
+  a.ldx = x_stride;
+  a.g = grad_y;
+  a.ldg = g_stride;
+  a.weight = weight;
+  a.y = grad_x;
+  a.stats = const_cast<float*>(stats);
+  a.grad_weight = grad_weight;
+  a.grad_bias = grad_bias;
+  if (norm && (grad_weight || grad_bias) && rows > 0) {
+    if (!workspace) return fail(AMBER_ERR_INVALID_ARGUMENT, "workspace is NULL");
+    if (workspace_bytes < amber_mpn_tail_backward_workspace_bytes(desc, rows, width))
+      return fail(AMBER_ERR_WORKSPACE_TOO_SMALL, "workspace %zu bytes, need %zu", workspace_bytes,
+                  amber_mpn_tail_backward_workspace_bytes(desc, rows, width));
+    a.partial = static_cast<float*>(workspace);
+  }
+  if (!grad_x && !grad_weight && !grad_bias) return AMBER_OK;
+  (void)hipGetLastError();
+  HIP_TRY(launch_tail_backward(a, norm, static_cast<hipStream_t>(stream)), "tail backward");
+  return AMBER_OK;
+}
+
 // workspace of amber_mpn_predict: [forward workspace | normalised x | normalised edge_attr]
 static size_t predict_norm_bytes(const AmberMpnDesc* d, int64_t N, int64_t E, size_t* xb_out) {
   const size_t xb = align256(sizeof(float) * static_cast<size_t>(N) * d->in_node_features);

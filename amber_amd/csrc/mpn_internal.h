@@ -329,4 +329,30 @@ hipError_t csr_build(const int64_t* edge_index, int64_t E, int64_t N, int32_t* r
 // this GPU's copy of the file-scope scratch array of csr.hip (AMBER_MPN_CSR_STATIC_SCRATCH_BYTES), 256-byte aligned
 hipError_t csr_static_scratch(void** out);
 
+// ---- activation -> LayerNorm -> dropout on rows (norm_dropout.hip) -----------------------------------------------------
+struct TailArgs {
+  int64_t rows, width;
+  const void* x;          // [rows, width], row stride ldx
+  int64_t ldx;
+  const void* g;          // backward: gradient of y, row stride ldg
+  int64_t ldg;
+  const void* weight;     // [width] or nullptr (ones)
+  const void* bias;       // [width] or nullptr (zeros)
+  void* y;                // forward: y, backward: gradient of x (or nullptr); dense
+  float* stats;           // [rows][2] mean, 1 / deviation
+  const int64_t* state;   // (seed, offset) of the generator
+  int64_t sequence;
+  float* partial;         // backward: [blocks][2][width] sums of the weight's and the bias's gradient, or nullptr
+  void* grad_weight;
+  void* grad_bias;
+  int32_t dtype, weight_dtype, act, drop;
+  uint32_t last_dropped;  // an element is dropped iff its word is <= this (drop != 0)
+  float scale, eps;
+};
+int64_t tail_partial_blocks(const TailArgs& a);  // rows of `partial` that the backward pass writes
+hipError_t launch_tail_forward(const TailArgs& a, bool normalize, hipStream_t s);
+hipError_t launch_tail_backward(const TailArgs& a, bool normalize, hipStream_t s);
+hipError_t launch_keep_mask(const TailArgs& a, uint8_t* out, hipStream_t s);
+hipError_t launch_generator_take(int64_t* state, int64_t count, int64_t* taken, hipStream_t s);
+
 }  // namespace amber

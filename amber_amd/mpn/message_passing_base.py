@@ -39,8 +39,9 @@ class MessagePassingBase(nn.Module):
     def __init__(self, *, in_node_features: int, in_edge_features: int, latent_dimension: int, stack_config: Dict,
                  embedding_config: Dict, output_type: str = "features", edge_dropout: float = 0.0,
                  create_graph_copy: bool = True, assert_graph_shapes: bool = True, device: Optional = None,
-                 node_type: str = "node"):
+                 node_type: str = "node", dropout_generator=None):
         super().__init__()
+        self.dropout_generator = dropout_generator  # CounterGenerator shared by edge and decoder dropout, or None: torch's
         self._latent_dimension = latent_dimension
         self._node_type = node_type
         self._in_node_features = in_node_features
@@ -52,7 +53,7 @@ class MessagePassingBase(nn.Module):
         if edge_dropout is not None and edge_dropout > 0.0:
             from amber_amd.mpn.common.edge_dropout import EdgeDropout
 
-            self.maybe_edge_dropout = EdgeDropout(dropout_prob=edge_dropout)
+            self.maybe_edge_dropout = EdgeDropout(dropout_prob=edge_dropout, generator=dropout_generator)
         else:
             self.maybe_edge_dropout = noop
         self._create_graph_copy = bool(create_graph_copy)

@@ -389,6 +389,54 @@ int amber_mpn_estimate_num_elements(const int64_t* simplices, int32_t verts_per_
                                     const int64_t* edges, int64_t num_mesh_edges, const double* positions, double gradation,
                                     double* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------
+ * The tail of a dense layer as stand-alone operators: activation -> LayerNorm -> dropout on rows [rows, width], any part of
+ * which may be absent, with its backward pass (what follows every Linear of the decoder MLP in train() mode,
+ * src/algorithm/architecture/mlp.py:58-96; LayerNorm alone and dropout alone are the same calls with the rest left out).
+ *
+ *   a = act(x);  n = (a - mean(a)) / sqrt(var(a) + eps);  y = dropout(n * weight + bias)       (normalize)
+ *   a = act(x);  y = dropout(a)                                                                (without)
+ *
+ * Random numbers come from a counter, not from a stored mask: element i (row-major) of a call owns word i & 3 of
+ * Philox-4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers, as easy as 1, 2, 3; SC 2011) under key = state[0] at
+ * counter words (lo, hi of i >> 2; lo, hi of state[1] + sequence).  It is dropped iff the word is < floor(p * 2^32) (every
+ * element for p = 1); a kept one is multiplied by float(1 / (1 - p)); a dropped one is +0 whatever it held (inf and NaN
+ * included), and so is its gradient.  The backward pass regenerates the same words.  `state` is a DEVICE int64[2] (seed,
+ * offset), so that a captured graph draws anew at every replay.
+ *
+ * amber_mpn_generator_take: taken = (state[0], state[1]) and state[1] += count, one atomic step (calls on several streams
+ * get disjoint ranges, in no fixed order).
+ * amber_mpn_keep_mask: out[i] = 1 where element i is kept, else 0.
+ * amber_mpn_tail_forward: x has row stride x_stride (elements; the features of a row are adjacent), y is dense.  stats:
+ * float[2 rows] (mean, 1 / sqrt(var + eps) of every row) for the backward pass, or NULL.  Without `normalize` x must be dense.
+ * amber_mpn_tail_backward: gradients from x, the forward's stats and grad_y (row stride g_stride; dense without `normalize`).
+ * grad_x (dense), grad_weight, grad_bias: any may be NULL.  x may be NULL when neither normalize nor an activation needs it.
+ * Sums over a row and over rows are in fp32 and in a fixed order: equal calls give equal bits.  Weights and their gradients are
+ * of weight_dtype (fp32, or x's own type); weight / bias may each be NULL (1 and 0).
+ * ------------------------------------------------------------------------------------------------- */
+enum { AMBER_DTYPE_F32 = 0, AMBER_DTYPE_BF16 = 1, AMBER_DTYPE_F16 = 2 };
+enum { AMBER_ACT_NONE = -1 };
+
+typedef struct AmberTailDesc {
+  int32_t dtype;        /* AMBER_DTYPE_* of x, y and their gradients */
+  int32_t weight_dtype; /* of weight, bias and their gradients: AMBER_DTYPE_F32 or dtype */
+  int32_t activation;   /* AMBER_ACT_* */
+  int32_t normalize;    /* 0 / 1 */
+  double p;             /* probability of an element being dropped, in [0, 1] */
+  double eps;           /* added to the variance, >= 0 */
+  int64_t sequence;     /* added to the state's offset, >= 0: several layers share one taken range */
+} AmberTailDesc;
+
+int amber_mpn_generator_take(int64_t* state, int64_t count, int64_t* taken, void* stream);
+int amber_mpn_keep_mask(const int64_t* state, int64_t sequence, double p, int64_t n, uint8_t* out, void* stream);
+int amber_mpn_tail_forward(const AmberTailDesc* desc, int64_t rows, int64_t width, const void* x, int64_t x_stride,
+                           const void* weight, const void* bias, const int64_t* state, void* y, float* stats, void* stream);
+size_t amber_mpn_tail_backward_workspace_bytes(const AmberTailDesc* desc, int64_t rows, int64_t width);
+int amber_mpn_tail_backward(const AmberTailDesc* desc, int64_t rows, int64_t width, const void* x, int64_t x_stride,
+                            const void* grad_y, int64_t g_stride, const void* weight, const float* stats, const int64_t* state,
+                            void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
 int amber_mpn_abi_version(void);
 const char* amber_mpn_last_error(void);
 
