@@ -183,6 +183,33 @@ def load() -> C.CDLL:
     return lib
 
 
+_binding = None
+
+
+def binding():
+    """The torch binding of the operators that are called often on little data (csrc/torch_binding.cpp), its calls bound to the
+    library that load() found.  Raises RuntimeError when it is missing: there is no fallback."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    lib = load()
+    import importlib.util
+    from importlib.machinery import ExtensionFileLoader
+
+    path = os.path.join(_HERE, "csrc", "amber_torch.so")
+    if not os.path.exists(path):
+        raise RuntimeError(f"amber_amd: torch binding not built ({path} missing). Run `make -C amber_amd/csrc` "
+                           f"(or __graft_entry__.build()). There is no fallback.")
+    loader = ExtensionFileLoader("amber_torch", path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("amber_torch", loader))
+    loader.exec_module(module)
+    module.bind(*(C.cast(getattr(lib, name), C.c_void_p).value
+                  for name in ("amber_mpn_last_error", "amber_mpn_generator_take", "amber_mpn_keep_mask", "amber_mpn_tail_forward",
+                               "amber_mpn_tail_backward_workspace_bytes", "amber_mpn_tail_backward")))
+    _binding = module
+    return module
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = load().amber_mpn_last_error()

@@ -290,7 +290,8 @@ def test_neighbours_of_the_outputs_stay(gpu_device):
     for dtype, rows, width in ((torch.float32, 5, 67), (torch.bfloat16, 3, 1031), (torch.float16, 70, 40), (torch.float32, 2, 17001)):
         n = rows * width
         x, w, b, go = (t.to(gpu_device) for t in _data(rows, width, dtype, dtype, seed=3))
-        desc = C.byref(_lib.AmberTailDesc(dtype=nd._DTYPES[dtype], weight_dtype=nd._DTYPES[dtype], activation=1, normalize=1, p=0.3,
+        name = _lib.DTYPE[str(dtype).split(".")[1]]
+        desc = C.byref(_lib.AmberTailDesc(dtype=name, weight_dtype=name, activation=1, normalize=1, p=0.3,
                                           eps=1e-5, sequence=0))
         state = _state(gpu_device)
         bufs = [torch.full((k + 128,), 7.0, dtype=t, device=gpu_device)
@@ -355,6 +356,16 @@ def test_refusals(gpu_device):
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y = nd.dropout(xr, 0.5, state)
         state.add_(1)  # the backward pass would draw other numbers
+        y.sum().backward()
+    for view in (lambda t: t, lambda t: t[:, 1:]):  # the input as well, read in place or not
+        base = xr * 2
+        y = nd.layer_norm(view(base))
+        base.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    y = nd.layer_norm(xr)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
         y.sum().backward()
 
 

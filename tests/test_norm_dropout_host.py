@@ -128,60 +128,53 @@ def test_python_refuses_cpu_tensors():
 
 
 def test_python_checks():
+    """Everything but the device is checked first, so a CPU tensor shows the refusals."""
+    x = torch.zeros(3, 4, dtype=torch.bfloat16)
+    state = torch.zeros(2, dtype=torch.int64)
     for p in (-0.1, 1.1, float("nan")):
-        with pytest.raises(ValueError, match="between 0 and 1"):
-            nd._check_p(p)
-    dev = torch.device("cpu")
-    with pytest.raises(ValueError, match="needs the generator"):
-        nd._check_state(None, dev)
+        for call in (lambda: nd.dropout(x, p, state), lambda: nd.keep_mask(4, p, state), lambda: nd.activate_norm_dropout(x, None, p=p)):
+            with pytest.raises(ValueError, match="between 0 and 1"):
+                call()
+    for call in (lambda: nd.dropout(x, 0.5), lambda: nd.keep_mask(4, 0.5, None), lambda: nd.activate_norm_dropout(x, None, p=0.5)):
+        with pytest.raises(ValueError, match="needs the generator"):
+            call()
     for bad in (torch.zeros(2), torch.zeros(3, dtype=torch.int64), torch.zeros(2, 2, dtype=torch.int64)[:, 0],
                 torch.zeros(1, 2, dtype=torch.int64)):
-        with pytest.raises(ValueError, match="contiguous int64"):
-            nd._check_state(bad, dev)
-    with pytest.raises(ValueError, match="the data on"):
-        nd._check_state(torch.zeros(2, dtype=torch.int64), torch.device("meta"))
+        for call in (lambda: nd.dropout(x, 0.5, bad), lambda: nd.keep_mask(4, 0.5, bad)):
+            with pytest.raises(ValueError, match="contiguous int64"):
+                call()
     for bad in (-1, 1 << 62):
-        with pytest.raises(ValueError, match="sequence"):
-            nd._check_sequence(bad)
+        for call in (lambda: nd.dropout(x, 0.5, state, sequence=bad), lambda: nd.keep_mask(4, 0.5, state, bad)):
+            with pytest.raises(ValueError, match="sequence"):
+                call()
     for bad in (-1e-5, float("nan"), float("inf")):
         with pytest.raises(ValueError, match="eps"):
-            nd._check_eps(bad)
-    x = torch.zeros(3, 4, dtype=torch.bfloat16)
-    assert nd._check_weights(x, None, None)[2] == torch.bfloat16
-    assert nd._check_weights(x, torch.ones(4), None)[2] == torch.float32
+            nd.layer_norm(x, eps=bad)
     with pytest.raises(ValueError, match="weight of shape"):
-        nd._check_weights(x, torch.ones(3), None)
+        nd.layer_norm(x, torch.ones(3))
     with pytest.raises(ValueError, match="bias of shape"):
-        nd._check_weights(x, None, torch.ones(1, 4))
+        nd.layer_norm(x, None, torch.ones(1, 4))
     with pytest.raises(TypeError, match="x's type"):
-        nd._check_weights(x, torch.ones(4, dtype=torch.float16), None)
+        nd.layer_norm(x, torch.ones(4, dtype=torch.float16))
     with pytest.raises(TypeError, match="weight is"):
-        nd._check_weights(x, torch.ones(4), torch.ones(4, dtype=torch.bfloat16))
+        nd.layer_norm(x, torch.ones(4), torch.ones(4, dtype=torch.bfloat16))
     with pytest.raises(ValueError, match="is on"):
-        nd._check_weights(x, torch.ones(4, device="meta"), None)
+        nd.layer_norm(x, torch.ones(4, device="meta"))
     for bad in (torch.tensor(1.0), torch.zeros(3, 0)):
         with pytest.raises(ValueError, match="last dimension"):
-            nd._check_weights(bad, None, None)
+            nd.layer_norm(bad)
+    for bad in (x.double(), x.long(), x.bool()):
+        with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+            nd.layer_norm(bad)
+    with pytest.raises(ValueError, match="Unknown activation"):
+        nd.activate_norm_dropout(x, "swiglu")
+    with pytest.raises(ValueError, match="without normalize"):
+        nd.activate_norm_dropout(x, "relu", torch.ones(4), normalize=False)
     with pytest.raises(ValueError, match="elements"):
-        nd.keep_mask(-1, 0.5, None)
-    with pytest.raises(ValueError, match="needs the generator"):
-        nd.keep_mask(4, 0.5, None)
-    with pytest.raises(ValueError, match="ranges"):
-        nd.CounterGenerator(1).take(0)
-
-
-def test_rows_reads_in_place_what_it_can():
-    base = torch.arange(60.0).reshape(10, 6)
-    for t, stride in ((base, 6), (base[:, 1:5], 6), (base[::2], 12), (base[::2, 2:], 12), (base.view(2, 5, 6)[:, :, :4], 6),
-                      (base[:1, 1:4], 3), (base[:, 2:3], 6), (base[:1].expand(7, 6), 0), (base.reshape(-1), 6)):
-        r, ld = nd._rows(t, t.shape[-1], False)
-        assert r.untyped_storage().data_ptr() == base.untyped_storage().data_ptr() and r.data_ptr() == t.data_ptr()
-        if t.dim() > 1 and t.shape[0] > 1:
-            assert ld == stride
-    for t in (base.t(), base[:, ::2], base[:, :1].expand(10, 6), base.view(2, 5, 6)[:, :4, :4], base.view(2, 5, 6).transpose(0, 1)):
-        r, ld = nd._rows(t, t.shape[-1], False)
-        assert ld == t.shape[-1] and torch.equal(r.reshape(t.shape), t) and r.is_contiguous()
-    assert nd._rows(base[:, :4], 4, True)[0].is_contiguous()  # dense rows asked for
+        nd.keep_mask(-1, 0.5, state)
+    for bad in (0, -1, 1 << 62):
+        with pytest.raises(ValueError, match="ranges"):
+            nd.CounterGenerator(1).take(bad)
 
 
 def test_generator_state_round_trip():
