@@ -65,7 +65,7 @@ __global__ __launch_bounds__(1024) void weight_gradient_kernel(TailArgs a, int64
 
 int64_t tail_partial_blocks(const TailArgs& a) {
   const Shape h = shape_for(a.width, vec_of(a.dtype));
-  return h.g ? backward_blocks(a, h) : blocks_for(a.rows, 1024);
+  return h.g ? backward_blocks(a, h) : blocks_for(a.rows, 256);
 }
 
 hipError_t launch_tail_forward(const TailArgs& a, bool normalize, hipStream_t s) {
