@@ -1472,7 +1472,7 @@ static int make_tail_args(const AmberTailDesc* d, int64_t rows, int64_t width, c
   if (!(d->eps >= 0.0 && d->eps <= 3.0e38)) return fail(AMBER_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
   if (d->sequence < 0) return fail(AMBER_ERR_INVALID_ARGUMENT, "negative sequence");
   if (rows < 0 || width < 0) return fail(AMBER_ERR_INVALID_ARGUMENT, "negative size");
-  if (width >= (1ll << 31) || (width > 0 && rows > (1ll << 50) / width))
+  if ((d->normalize && width > (1ll << 30)) || (width > 0 && rows > (1ll << 50) / width) || width > (1ll << 50))
     return fail(AMBER_ERR_INVALID_ARGUMENT, "rows / width out of range");
   if (d->normalize && width == 0) return fail(AMBER_ERR_INVALID_ARGUMENT, "LayerNorm over no features");
   a = TailArgs{};

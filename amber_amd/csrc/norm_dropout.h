@@ -352,10 +352,13 @@ DEVINL void join_waves(float (&v)[N], float (&box)[W][N]) {
     for (int w = 1; w < W; ++w) v[i] += box[w][i];
   }
 }
-// 1 / sqrt(v): the hardware's estimate (1 unit in the last place) and one Newton step
+// 1 / sqrt(v): the hardware's estimate (1 unit in the last place) and one Newton step.  The estimate takes no subnormal numbers,
+// the step no infinity: a variance below 2^-96 is scaled, an overflown one gives 0.
 DEVINL float rsqrt_of(float v) {
-  const float r = __builtin_amdgcn_rsqf(v);
-  return r * fmaf(-0.5f * v * r, r, 1.5f);
+  const bool tiny = v < 0x1p-96f;
+  const float u = tiny ? v * 0x1p96f : v, r = __builtin_amdgcn_rsqf(u);
+  const float q = r * fmaf(-0.5f * u * r, r, 1.5f);
+  return u > 3.0e38f ? r : tiny ? q * 0x1p48f : q;
 }
 // sum / D with inv = 1 / D rounded: one correction, so that a row of equal values has exactly that value as its mean
 DEVINL float mean_of(float sum, float width, float inv) {

@@ -90,6 +90,13 @@ Rows rows_of(const Tensor& t, int64_t width, bool dense) {
   return {t.contiguous(), width};
 }
 
+// What the kernels read through a pointer has to be there as written: negation bits and zero tensors without memory are resolved.
+Tensor plain(const Tensor& t) {
+  if (!t.defined()) return t;
+  if (t._is_zerotensor()) return t.clone();
+  return t.is_neg() ? t.resolve_neg() : t;
+}
+
 const void* data(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* mutable_data(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 
@@ -111,15 +118,15 @@ struct TailBackward : public torch::autograd::Node {
 
   variable_list apply(variable_list&& grads) override {
     variable_list out(3);
-    const Tensor& grad_y = grads[0];
-    if (!grad_y.defined()) return out;
+    if (!grads[0].defined()) return out;
     {
       std::lock_guard<std::mutex> lock(mutex_);
       const Tensor xs = x.unpack(), ws = weight.unpack(), ss = stats.unpack(), st = state.unpack();
       at::AutoDispatchBelowADInplaceOrView below;
-      const c10::DeviceGuard guard(grad_y.device());
+      const c10::DeviceGuard guard(grads[0].device());
+      const Tensor grad_y = plain(grads[0]);
       const bool normalize = desc.normalize != 0;
-      const int64_t width = grad_y.dim() ? grad_y.size(-1) : 1, rows = width ? grad_y.numel() / width : 0;
+      const int64_t width = normalize ? grad_y.size(-1) : 1, rows = grad_y.numel() / width;
       const Rows g = rows_of(grad_y, width, !normalize);
       const bool need_w = task_should_compute_output(1), need_b = task_should_compute_output(2);
       if (task_should_compute_output(0)) out[0] = at::empty(grad_y.sizes(), grad_y.options());
@@ -145,10 +152,15 @@ struct TailBackward : public torch::autograd::Node {
   }
 };
 
+void no_forward_mode(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), "amber_amd: forward-mode derivatives are not built");
+}
+
 // y = dropout(layer_norm(act(x))), any part absent.  p is 0 outside training.
-Tensor tail(const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, const std::optional<Tensor>& state_,
+Tensor tail(const Tensor& x_, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, const std::optional<Tensor>& state_,
             int64_t activation, bool normalize, double p, double eps, int64_t sequence) {
   AmberTailDesc desc{};
+  const Tensor x = plain(x_);
   TORCH_CHECK_TYPE(dtype_id(x.scalar_type(), desc.dtype), "amber_amd: x must be float32, bfloat16 or float16, got ", x.scalar_type());
   check_probability(p);
   check_sequence(sequence);
@@ -167,7 +179,7 @@ Tensor tail(const Tensor& x, const std::optional<Tensor>& weight_, const std::op
       TORCH_CHECK_VALUE(from->device() == x.device(), "amber_amd: ", name, " is on ", from->device(), ", x on ", x.device());
       TORCH_CHECK_TYPE(from->scalar_type() == x.scalar_type() || from->scalar_type() == at::kFloat, "amber_amd: ", name,
                        " must be of x's type (", x.scalar_type(), ") or float32, got ", from->scalar_type());
-      to = *from;
+      to = plain(*from);
       weight_type = to.scalar_type();
     };
     take(weight_, "weight", weight);
@@ -183,7 +195,10 @@ Tensor tail(const Tensor& x, const std::optional<Tensor>& weight_, const std::op
     check_state_device(*state_, x.device());
     state = *state_;
   }
-  if (!normalize && !drops && activation == AMBER_ACT_NONE) return x;
+  if (!normalize && !drops && activation == AMBER_ACT_NONE) return x_;
+  no_forward_mode(x);
+  no_forward_mode(weight);
+  no_forward_mode(bias);
   dtype_id(weight_type, desc.weight_dtype);
   desc.activation = static_cast<int32_t>(activation);
   desc.normalize = normalize;
@@ -198,7 +213,7 @@ Tensor tail(const Tensor& x, const std::optional<Tensor>& weight_, const std::op
   {
     at::AutoDispatchBelowADInplaceOrView below;
     const c10::DeviceGuard guard(x.device());
-    const int64_t width = x.dim() ? x.size(-1) : 1, rows = width ? x.numel() / width : 0;
+    const int64_t width = normalize ? x.size(-1) : 1, rows = x.numel() / width;  // without the norm: one flat row of elements
     r = rows_of(x, width, !normalize);
     if (weight.defined()) w = weight.contiguous();
     const Tensor b = bias.defined() ? bias.contiguous() : bias;
@@ -245,6 +260,7 @@ Tensor generator_take(const Tensor& state, int64_t count) {
   check_device(state, "generator state");
   const c10::DeviceGuard guard(state.device());
   const Tensor taken = at::empty_like(state);
+  state.unsafeGetTensorImpl()->bump_version();  // a backward pass that reads the generator's own buffer instead of `taken` must notice
   check(g_lib.take(state.mutable_data_ptr<int64_t>(), count, taken.mutable_data_ptr<int64_t>(), stream_of(state.device())), "generator take");
   return taken;
 }

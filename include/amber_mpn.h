@@ -407,6 +407,7 @@ int amber_mpn_estimate_num_elements(const int64_t* simplices, int32_t verts_per_
  * amber_mpn_generator_take: taken = (state[0], state[1]) and state[1] += count, one atomic step (calls on several streams
  * get disjoint ranges, in no fixed order).
  * amber_mpn_keep_mask: out[i] = 1 where element i is kept, else 0.
+ * Sizes: width <= 2^30 with `normalize`, rows * width <= 2^50.
  * amber_mpn_tail_forward: x has row stride x_stride (elements; the features of a row are adjacent), y is dense.  stats:
  * float[2 rows] (mean, 1 / sqrt(var + eps) of every row) for the backward pass, or NULL.  Without `normalize` x must be dense.
  * amber_mpn_tail_backward: gradients from x, the forward's stats and grad_y (row stride g_stride; dense without `normalize`).

@@ -220,6 +220,14 @@ def test_constant_and_extreme_rows(gpu_device):
     for value in (0.0, 1.0, -3.75, 2.0 ** 60):  # sums of 100 equal powers-of-two multiples are exact: variance 0, y = bias
         assert torch.equal(nd.layer_norm(torch.full((3, 100), value, device=gpu_device), w, b), b.expand(3, 100))
     assert bool(torch.isnan(nd.layer_norm(torch.zeros(2, 8, device=gpu_device), eps=0.0)).all())  # 0 / 0, as torch
+    # no eps and a variance far below the smallest normal number, or one that overflows (1 / sqrt(inf) = 0: the bias alone)
+    x = torch.randn(7, 100, generator=torch.Generator().manual_seed(3))
+    want = orc.tail(x, eps=0.0)[0]
+    for scale in (2.0 ** -66, 2.0 ** -50, 1.0, 2.0 ** 50):
+        got = nd.layer_norm((x * scale).to(gpu_device), eps=0.0).cpu().double()
+        # below 2^-126 the variance itself has fewer bits: 2^-132 keeps 17 of them, half of that relative error reaches y
+        assert float((got - want).abs().max()) <= (64 * U if scale > 2.0 ** -60 else 2.0 ** -16) * float(want.abs().max()), scale
+    assert torch.equal(nd.layer_norm((x * 1e25).to(gpu_device), w, b), b.expand(7, 100))
     # a large common offset: the variance is formed from differences, not from squares.  Offset 4096 + k / 4 is exact in fp32,
     # the mean of 64 such values too
     x = 4096.0 + torch.arange(64.0).repeat(5, 1) / 4
@@ -386,6 +394,46 @@ def test_gradients_against_differences(gpu_device):
             lo, hi = ([t + s * h * v if i == k else t for i, t in enumerate(d[:3])] for s in (-1, 1))
             diff = (f(*hi) - f(*lo)) / (2 * h)
             assert abs(diff - float((grads[k].double() * v.double()).sum())) <= 0.01 * float(grads[k].double().norm()), (act, k)
+
+
+def test_zero_and_negated_tensors(gpu_device):
+    """Tensors whose memory does not hold their values: a negated view, a gradient of zeros without memory."""
+    x = torch.randn(6, 40, dtype=torch.complex64, device=gpu_device).conj().imag
+    assert x.is_neg()
+    assert torch.equal(nd.layer_norm(x), nd.layer_norm(x.clone())) and torch.equal(nd.dropout(x, 0.3, _state(gpu_device)),
+                                                                                   nd.dropout(x.clone(), 0.3, _state(gpu_device)))
+    xr, w = torch.randn(6, 40, device=gpu_device, requires_grad=True), torch.randn(40, device=gpu_device, requires_grad=True)
+    zero = torch._efficientzerotensor((6, 40), device=gpu_device)
+    gx, gw = torch.autograd.grad(nd.layer_norm(xr, w), (xr, w), zero)
+    assert not bool(gx.any()) and not bool(gw.any())
+    y = nd.layer_norm(xr, w)
+    g = torch.randn(6, 40, dtype=torch.complex64, device=gpu_device).conj().imag
+    a = torch.autograd.grad(y, (xr, w), g, retain_graph=True)
+    assert all(torch.equal(s, t) for s, t in zip(a, torch.autograd.grad(y, (xr, w), g.clone())))  # and twice through one graph
+
+
+def test_generator_buffer_as_state_is_guarded(gpu_device):
+    gen = nd.CounterGenerator(3, device=gpu_device)
+    x = torch.randn(5, 5, device=gpu_device, requires_grad=True)
+    y = nd.dropout(x, 0.5, gen.state)
+    gen.take()  # moves the offset that the backward pass would read
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_forward_mode_is_refused(gpu_device):
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn(4, 8, device=gpu_device)
+    with fwd.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            nd.layer_norm(fwd.make_dual(x, torch.ones_like(x)))
+
+
+def test_one_dimension_beyond_32_bits(gpu_device):
+    n = (1 << 32) + 7
+    x = torch.ones(n, dtype=torch.bfloat16, device=gpu_device)
+    y = nd.dropout(x, 0.5, _state(gpu_device))
+    assert torch.equal(y[-11:].cpu(), orc.keep(11, 0.5, 1234567890123, 17, start=n - 11).to(torch.bfloat16) * 2)
 
 
 def test_offsets_beyond_32_bits(gpu_device):

@@ -67,7 +67,8 @@ def _tail_desc(**kw):
     ({}, 4, -8, -1, b"negative size"),
     ({}, 4, 0, -1, b"no features"),
     ({}, 1 << 40, 1 << 20, -1, b"out of range"),
-    ({}, 1, 1 << 31, -1, b"out of range"),
+    ({}, 1, (1 << 30) + 1, -1, b"out of range"),
+    (dict(normalize=0), 1, (1 << 50) + 1, -1, b"out of range"),
     (dict(p=0.5), 4, 8, -1, b"state is NULL"),
     ({}, 4, 8, -1, b"x / y is NULL"),
 ])
