@@ -609,7 +609,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_forward(TailA
 
 // Needs x, the gradient and two statistics of a row; the gradients of weight and bias gather in registers over a team's rows and
 // are joined over the block at its end.  W = 16 (rows beyond 8192 features) has 128 registers a lane: it fetches a row when it
-// needs it and the weights once per row (10000 x 12000 fp32: 625 us with both kept, spilled to memory).
+// needs it, reads x once more from the cache for the second half and the weights once per row (10000 x 12000 fp32: 323 us, 625 with
+// all of it kept and spilled to memory).  Two rows on their way instead of one changed nothing (20000 x 8192 fp32 381 us, 385).
 template <class T, int G, int W, int K, bool SMOOTH>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(TailArgs a) {
   constexpr int V = kVec<T>, LANES = G * W, THREADS = W == 1 ? 256 : 64 * W, TEAMS = THREADS / LANES;
@@ -657,7 +658,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(Tail
     for (int k = 0; k < K; ++k) {
       if (k == K - 1 && !last) break;
       if (a.drop) drop_pack(a, s, row * cols.width + cols.at[k], h[k]);
-      act_pack<SMOOTH, true>(a.act, n[k], dact[k]);
+      if (LEAN) act_pack<SMOOTH, false>(a.act, n[k], n[k]);
+      else act_pack<SMOOTH, true>(a.act, n[k], dact[k]);
       float(&wk)[V] = w[LEAN ? 0 : k];
       if (LEAN) cols.load_weight_pack(a.weight, fp32, 1.f, k, wk);
 #pragma unroll
@@ -689,12 +691,21 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(Tail
     if (!a.y) continue;
     T* y = static_cast<T*>(a.y) + row * cols.width;
     const float m0 = sums[0] * inv, m1 = sums[1] * inv;
+    if (LEAN) cols.load(x + row * a.ldx, xn);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (k == K - 1 && !last) break;
       float d[V];
+      if (LEAN) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) d[j] = rstd * (h[k][j] - m0 - n[k][j] * m1) * dact[k][j];
+        for (int j = 0; j < V; ++j) n[k][j] = to_f(xn[k][j]);
+        act_pack<SMOOTH, true>(a.act, n[k], d);
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[j] *= rstd * (h[k][j] - m0 - (n[k][j] - mean) * rstd * m1);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[j] = rstd * (h[k][j] - m0 - n[k][j] * m1) * dact[k][j];
+      }
       cols.store(y, k, d);
     }
   }
@@ -749,6 +760,7 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct Shape {
   int g, w, k;
 };
+inline int vec_of(int dtype) { return dtype == AMBER_DTYPE_F32 ? 4 : 8; }
 inline Shape shape_for(int64_t width, int vec) {
   if (width < vec) return {1, 1, 1};
   const int64_t packs = cdiv(width, vec);
@@ -760,23 +772,29 @@ inline Shape shape_for(int64_t width, int vec) {
       if (packs <= 64 * w * k) return {64, w, k};
   return {0, 0, 0};
 }
-inline int vec_of(int dtype) { return dtype == AMBER_DTYPE_F32 ? 4 : 8; }
 inline int64_t teams_in_block(const Shape& h) { return h.w > 1 ? 1 : 256 / h.g; }
-// Blocks of a launch: each takes rows in turn, so this sets how many rows are in flight.  More waves than the memory needs only
-// spread the accesses: 1.44 M x 128 fp32 forward runs at 250 us with 1024 blocks (5.9 TB/s), 311 with 512, 328 with 2048; 100000 x
-// 1024 fp32 backward at 219 with 256, 237 with 1024.  The generator's arithmetic asks for more of them: 100000 x 2048 bf16 forward
-// with dropout 292 us with 512 blocks, 185 with 1280 (without it 142 with 1024, 144 with 1280).  Measured from 32 to 16384
-// features, 1000 to 2 M rows, fp32 and bf16, with and without dropout, in steps of 256 blocks; the rule is within 6 % of the best.
+// Blocks of a launch: each takes rows in turn and has the next ones on their way, so their number sets the bytes in flight.  About
+// 4 MB forward and 6 MB backward (x and the gradient) are best; more only spread the accesses over more pages: 1.44 M x 128 fp32
+// forward 250 us with 1024 blocks (5.9 TB/s), 311 with 512, 328 with 2048; 100000 x 1024 fp32 backward 219 with 256, 237 with 1024.
+// The generator and the smooth activations ask for more waves than that: 100000 x 2048 bf16 forward with dropout 292 us with 512
+// blocks, 185 with 1280; 100000 x 1024 fp32 184 with 256, 154 with 768.  Measured from 32 to 16384 features, 1000 to 2 M rows, fp32
+// and bf16, with and without dropout, in steps of 256 blocks: a CU more or less than the others counts (100000 x 1020 fp32 forward
+// 136 us with 256 blocks, 175 with 257).  Backward teams of 8 and 16 waves fit once on a CU.
+inline int64_t clamped(int64_t v, int64_t low, int64_t high) { return v < low ? low : v > high ? high : v; }
+inline int64_t even(int64_t blocks) { return (blocks + 128) / 256 * 256; }  // a whole number of them on each of the 256 CUs
+inline int64_t block_bytes(const TailArgs& a, const Shape& h) { return teams_in_block(h) * a.width * (16 / vec_of(a.dtype)); }
 inline int64_t forward_blocks(const TailArgs& a, const Shape& h) {
-  int64_t most = h.k == 1 ? 1024 : 512;
-  if (a.drop && (h.k > 1 || a.dtype != AMBER_DTYPE_F32)) most = h.w >= 8 ? 1024 : 1280;
-  return blocks_for(cdiv(a.rows, teams_in_block(h)), most);
+  const bool half = a.dtype != AMBER_DTYPE_F32;
+  const int64_t least = a.drop && half ? 1280 : a.drop || is_smooth(a.act) ? 768 : 256;
+  return blocks_for(cdiv(a.rows, teams_in_block(h)), clamped(even((4 << 20) / block_bytes(a, h)), least, 2048));
 }
 inline int64_t backward_blocks(const TailArgs& a, const Shape& h) {
-  const int64_t most = h.k == 1 ? 768 : h.w >= 8 || h.k > 2 ? 256 : 512;
+  const bool half = a.dtype != AMBER_DTYPE_F32;
+  const int64_t least = a.drop && half && h.w < 8 ? 512 : 256;
+  int64_t blocks = clamped(even((6 << 20) / (2 * block_bytes(a, h))), least, h.w < 8 ? 768 : 256);
   if (h.w > 1)  // a block's partial sums cost 8 bytes a feature each way: at least 16 rows a block
-    return blocks_for(a.rows, a.rows / 16 < 256 ? 256 : a.rows / 16 < most ? a.rows / 16 : most);
-  return blocks_for(cdiv(a.rows, teams_in_block(h)), most);
+    blocks = clamped(even(a.rows / 16), 256, blocks);
+  return blocks_for(cdiv(a.rows, teams_in_block(h)), blocks);
 }
 
 template <class T, int G, int W, int K, bool SMOOTH>
