@@ -607,16 +607,17 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_forward(TailA
   }
 }
 
-// Needs x, the gradient and two statistics of a row; the gradients of weight and bias gather in registers over a team's rows and
-// are joined over the block at its end.  W = 16 (rows beyond 8192 features) has 128 registers a lane: it fetches a row when it
-// needs it, reads x once more from the cache for the second half and the weights once per row (10000 x 12000 fp32: 323 us, 625 with
-// all of it kept and spilled to memory).  Two rows on their way instead of one changed nothing (20000 x 8192 fp32 381 us, 385).
+// Needs x, the gradient and two statistics of a row; the gradients of weight and bias gather over a team's rows, in registers (W = 16,
+// rows beyond 8192 features: 128 registers a lane are too few, so in LDS, where every thread adds to places of its own), and are
+// joined over the block at its end.  Two rows on their way instead of one changed nothing (20000 x 8192 fp32 381 us, 385).
 template <class T, int G, int W, int K, bool SMOOTH>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(TailArgs a) {
   constexpr int V = kVec<T>, LANES = G * W, THREADS = W == 1 ? 256 : 64 * W, TEAMS = THREADS / LANES;
-  constexpr bool LEAN = W == 16;
+  constexpr bool IN_LDS = W == 16, AHEAD = !(IN_LDS && K * V == 16);
   __shared__ float box[2][W][2];
-  __shared__ float columns[W == 1 ? 2 * LANES * K * V : 1];
+  // W = 1: [2][columns] for the join of the block's waves; IN_LDS: [2][K][V / 4][threads] packs of 4 sums
+  __shared__ __attribute__((aligned(16))) float columns[W == 1 || IN_LDS ? 2 * LANES * K * V : 4];
+  Pack<float>* const mine = reinterpret_cast<Pack<float>*>(columns) + threadIdx.x;
   const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
   const Columns<T, LANES, K, LANES == 1> cols(lane, static_cast<int>(a.width));
   const bool ragged = cols.ragged(), last = W == 1 || __any(cols.stores(K - 1)), fp32 = a.weight_dtype == AMBER_DTYPE_F32;
@@ -633,17 +634,22 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(Tail
     mean_next = a.stats[2 * r];
     rstd_next = a.stats[2 * r + 1];
   };
-  if (!LEAN && row < a.rows) fetch(row);
+  if (AHEAD && row < a.rows) fetch(row);
   Stream s{};
   if (a.drop) s = stream_of(a.state, a.sequence);
-  float w[LEAN ? 1 : K][V], dw[K][V], db[K][V];
-  if constexpr (!LEAN) cols.load_weights(a.weight, fp32, 1.f, w);
+  float w[K][V], dw[IN_LDS ? 1 : K][V], db[IN_LDS ? 1 : K][V];
+  cols.load_weights(a.weight, fp32, 1.f, w);
+  if (IN_LDS) {
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+    for (int i = 0; i < 2 * K * V / 4; ++i) mine[i * THREADS] = Pack<float>{0.f, 0.f, 0.f, 0.f};
+  } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) dw[k][j] = db[k][j] = 0.f;
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) dw[IN_LDS ? 0 : k][j] = db[IN_LDS ? 0 : k][j] = 0.f;
+  }
   for (int turn = 0; row < a.rows; row += stride, turn ^= 1) {
-    if (LEAN) fetch(row);
+    if (!AHEAD) fetch(row);
     const float mean = mean_next, rstd = rstd_next;
     float n[K][V], h[K][V], dact[K][V], sums[2] = {0.f, 0.f};
 #pragma unroll
@@ -653,22 +659,35 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(Tail
         n[k][j] = to_f(xn[k][j]);
         h[k][j] = to_f(gn[k][j]);
       }
-    if (!LEAN && row + stride < a.rows) fetch(row + stride);
+    if (AHEAD && row + stride < a.rows) fetch(row + stride);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (k == K - 1 && !last) break;
       if (a.drop) drop_pack(a, s, row * cols.width + cols.at[k], h[k]);
-      if (LEAN) act_pack<SMOOTH, false>(a.act, n[k], n[k]);
-      else act_pack<SMOOTH, true>(a.act, n[k], dact[k]);
-      float(&wk)[V] = w[LEAN ? 0 : k];
-      if (LEAN) cols.load_weight_pack(a.weight, fp32, 1.f, k, wk);
+      act_pack<SMOOTH, true>(a.act, n[k], dact[k]);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        n[k][j] = (n[k][j] - mean) * rstd;
-        dw[k][j] += h[k][j] * n[k][j];
-        db[k][j] += h[k][j];
-        h[k][j] *= wk[j];
+      for (int j = 0; j < V; ++j) n[k][j] = (n[k][j] - mean) * rstd;
+      if (IN_LDS) {
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+          Pack<float> tw = mine[(k * (V / 4) + q) * THREADS], tb = mine[((K + k) * (V / 4) + q) * THREADS];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            tw[j] += h[k][4 * q + j] * n[k][4 * q + j];
+            tb[j] += h[k][4 * q + j];
+          }
+          mine[(k * (V / 4) + q) * THREADS] = tw;
+          mine[((K + k) * (V / 4) + q) * THREADS] = tb;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          dw[IN_LDS ? 0 : k][j] += h[k][j] * n[k][j];
+          db[IN_LDS ? 0 : k][j] += h[k][j];
+        }
       }
+#pragma unroll
+      for (int j = 0; j < V; ++j) h[k][j] *= w[k][j];
       if (k < K - 1 || !ragged) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -691,34 +710,25 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(Tail
     if (!a.y) continue;
     T* y = static_cast<T*>(a.y) + row * cols.width;
     const float m0 = sums[0] * inv, m1 = sums[1] * inv;
-    if (LEAN) cols.load(x + row * a.ldx, xn);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (k == K - 1 && !last) break;
       float d[V];
-      if (LEAN) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) n[k][j] = to_f(xn[k][j]);
-        act_pack<SMOOTH, true>(a.act, n[k], d);
-#pragma unroll
-        for (int j = 0; j < V; ++j) d[j] *= rstd * (h[k][j] - m0 - (n[k][j] - mean) * rstd * m1);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) d[j] = rstd * (h[k][j] - m0 - n[k][j] * m1) * dact[k][j];
-      }
+      for (int j = 0; j < V; ++j) d[j] = rstd * (h[k][j] - m0 - n[k][j] * m1) * dact[k][j];
       cols.store(y, k, d);
     }
   }
   if (!a.partial) return;
   float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * cols.width;
-  if (W > 1) {
+  if constexpr (W > 1) {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (cols.counts(k, j)) {
-          out[cols.at[k] + j] = dw[k][j];
-          out[cols.width + cols.at[k] + j] = db[k][j];
+          out[cols.at[k] + j] = IN_LDS ? mine[(k * (V / 4) + j / 4) * THREADS][j % 4] : dw[IN_LDS ? 0 : k][j];
+          out[cols.width + cols.at[k] + j] = IN_LDS ? mine[((K + k) * (V / 4) + j / 4) * THREADS][j % 4] : db[IN_LDS ? 0 : k][j];
         }
     return;
   }
