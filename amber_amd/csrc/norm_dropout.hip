@@ -37,28 +37,42 @@ __global__ __launch_bounds__(kBlock) void keep_mask_kernel(TailArgs a, uint8_t* 
   }
 }
 
-// gradients of weight and bias: the blocks' partial sums [blocks][2 width].  A block takes 16 columns, 64 threads each of them:
-// thread q adds blocks q, q + 64, ... in order, then a tree over q.
+// gradients of weight and bias: the blocks' partial sums [blocks][2 width].  A block of 1024 threads takes C columns, Q = 1024 / C
+// threads each: thread q adds blocks q, q + Q, ... in order, then a tree over q (always the same one).  Few columns are cut small, so
+// that more than a handful of CUs works on them; many wide, for whole cache lines (16 for all: 768 x 128 4.1 us, now 3.5; 256 x 8198
+// 6.6, now 4.7; 256 x 16384 8.0, now 5.0).  A launch of its own: a last block that joins would need a counter that someone clears.
+template <int C>
 __global__ __launch_bounds__(1024) void weight_gradient_kernel(TailArgs a, int64_t blocks) {
-  __shared__ float box[16][65];
-  const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
-  const int64_t column = static_cast<int64_t>(blockIdx.x) * 16 + c, columns = 2 * a.width;
+  constexpr int Q = 1024 / C, LANES = Q < 64 ? Q : 64, PER = Q / LANES;
+  __shared__ float box[C][Q + 1];
+  const int c = threadIdx.x % C, q = threadIdx.x / C;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * C, columns = 2 * a.width;
   float sum = 0.f;
-  if (column < columns) {
+  if (first + c < columns) {
+    const float* p = a.partial + q * columns + first + c;
 #pragma unroll 8
-    for (int64_t b = q; b < blocks; b += 64) sum += a.partial[b * columns + column];
+    for (int64_t b = q; b < blocks; b += Q, p += Q * columns) sum += *p;
   }
   box[c][q] = sum;
   __syncthreads();
-  const int wave = threadIdx.x >> 6;
-  sum = team_sum<64>(box[wave][threadIdx.x & 63]);
-  const int64_t out = static_cast<int64_t>(blockIdx.x) * 16 + wave;
-  if ((threadIdx.x & 63) != 0 || out >= columns) return;
+  const int mine = threadIdx.x / LANES, lane = threadIdx.x % LANES;  // LANES lanes join a column
+  if (mine >= C) return;
+  sum = box[mine][lane];
+#pragma unroll
+  for (int i = 1; i < PER; ++i) sum += box[mine][lane + i * LANES];
+  sum = team_sum<LANES>(sum);
+  const int64_t out = first + mine;
+  if (lane != 0 || out >= columns) return;
   void* to = out < a.width ? a.grad_weight : a.grad_bias;
   const int64_t i = out < a.width ? out : out - a.width;
   if (a.weight_dtype == AMBER_DTYPE_F32) store_weight<float>(to, 1, i, sum);
   else if (a.weight_dtype == AMBER_DTYPE_BF16) store_weight<bf16>(to, 0, i, sum);
   else store_weight<f16>(to, 0, i, sum);
+}
+template <int C>
+void launch_weight_gradient(const TailArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((weight_gradient_kernel<C>), dim3(static_cast<unsigned>(cdiv(2 * a.width, C))), dim3(1024), 0, s, a,
+                     a.rows > 0 ? tail_partial_blocks(a) : 0);
 }
 
 }  // namespace
@@ -85,9 +99,11 @@ hipError_t launch_tail_backward(const TailArgs& a, bool normalize, hipStream_t s
     }
     if (e != hipSuccess) return e;
   }
-  if (a.grad_weight || a.grad_bias)  // no rows: zeros
-    hipLaunchKernelGGL(weight_gradient_kernel, dim3(static_cast<unsigned>(cdiv(2 * a.width, 16))), dim3(1024), 0, s, a,
-                       a.rows > 0 ? tail_partial_blocks(a) : 0);
+  if (a.grad_weight || a.grad_bias) {  // no rows: zeros
+    if (a.width <= 256) launch_weight_gradient<4>(a, s);
+    else if (a.width <= 1024) launch_weight_gradient<16>(a, s);
+    else launch_weight_gradient<64>(a, s);
+  }
   return hipGetLastError();
 }
 hipError_t launch_keep_mask(const TailArgs& a, uint8_t* out, hipStream_t s) {

@@ -139,11 +139,12 @@ def test_layer_norm_forward_backward(gpu_device, shape, types):
                          ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else str(v))
 def test_activate_norm_dropout(gpu_device, shape, types, p, act, normalize):
     dtype, wdtype = (DTYPES[t] for t in types.split("-"))
-    if act is None and not normalize and p == 0.0:
-        pytest.skip("the identity")
     x, w, b, go = _data(*shape, dtype, wdtype, seed=shape[1] + 1)
     kept = orc.keep(x.numel(), p, 1234567890123, 17 + 3).view(shape) if p > 0 else None
     d = [t.to(gpu_device) for t in (x, w, b, go)]
+    if act is None and not normalize and p == 0.0:
+        assert nd.activate_norm_dropout(d[0], None, normalize=False) is d[0]  # nothing to do
+        return
     got = _run(d[0], act, d[1], d[2], normalize, p, _state(gpu_device), d[3], sequence=3)
     args = (act, w, b) if normalize else (act, None, None)
     _compare(got, orc.tail(x, *args, normalize=normalize, kept=kept, p=p, grad=go),
@@ -328,7 +329,7 @@ def test_empty_batches(gpu_device):
     assert d.shape == (5, 0) and torch.autograd.grad(d, z, torch.empty(5, 0, device=gpu_device))[0].shape == (5, 0)
     assert nd.keep_mask(0, 0.5, state).shape == (0,)
     s = torch.tensor(3.0, device=gpu_device, requires_grad=True)  # no dimensions: one element
-    assert nd.dropout(s, 1.0, state).shape == () and float(nd.dropout(s, 1.0, state)) == 0.0
+    assert nd.dropout(s, 1.0, state).shape == () and float(nd.dropout(s, 1.0, state).detach()) == 0.0
 
 
 def test_identities(gpu_device):
