@@ -1536,8 +1536,7 @@ int amber_mpn_tail_forward(const AmberTailDesc* desc, int64_t rows, int64_t widt
 size_t amber_mpn_tail_backward_workspace_bytes(const AmberTailDesc* desc, int64_t rows, int64_t width) {
   TailArgs a;
   if (make_tail_args(desc, rows, width, nullptr, false, a)) return 0;
-  if (!desc->normalize || rows == 0) return 256;
-  return align256(sizeof(float) * 2 * static_cast<size_t>(width) * static_cast<size_t>(tail_partial_blocks(a))) + 256;
+  return desc->normalize ? align256(sizeof(float) * static_cast<size_t>(tail_partial_floats(a))) : 0;
 }
 
 int amber_mpn_tail_backward(const AmberTailDesc* desc, int64_t rows, int64_t width, const void* x, int64_t x_stride,
@@ -1569,11 +1568,10 @@ int amber_mpn_tail_backward(const AmberTailDesc* desc, int64_t rows, int64_t wid
   a.stats = const_cast<float*>(stats);
   a.grad_weight = grad_weight;
   a.grad_bias = grad_bias;
-  if (norm && (grad_weight || grad_bias) && rows > 0) {
+  const size_t need = norm && (grad_weight || grad_bias) ? align256(sizeof(float) * static_cast<size_t>(tail_partial_floats(a))) : 0;
+  if (need) {
     if (!workspace) return fail(AMBER_ERR_INVALID_ARGUMENT, "workspace is NULL");
-    if (workspace_bytes < amber_mpn_tail_backward_workspace_bytes(desc, rows, width))
-      return fail(AMBER_ERR_WORKSPACE_TOO_SMALL, "workspace %zu bytes, need %zu", workspace_bytes,
-                  amber_mpn_tail_backward_workspace_bytes(desc, rows, width));
+    if (workspace_bytes < need) return fail(AMBER_ERR_WORKSPACE_TOO_SMALL, "workspace %zu bytes, need %zu", workspace_bytes, need);
     a.partial = static_cast<float*>(workspace);
   }
   if (!grad_x && !grad_weight && !grad_bias) return AMBER_OK;

@@ -342,14 +342,15 @@ struct TailArgs {
   float* stats;           // [rows][2] mean, 1 / deviation
   const int64_t* state;   // (seed, offset) of the generator
   int64_t sequence;
-  float* partial;         // backward: [blocks][2][width] sums of the weight's and the bias's gradient, or nullptr
+  float* partial;         // backward: [blocks][2][width] sums of the weight's and the bias's gradient, or nullptr (one block, or none wanted)
   void* grad_weight;
   void* grad_bias;
   int32_t dtype, weight_dtype, act, drop;
   uint32_t last_dropped;  // an element is dropped iff its word is <= this (drop != 0)
   float scale, eps;
 };
-int64_t tail_partial_blocks(const TailArgs& a);  // rows of `partial` that the backward pass writes
+int64_t tail_partial_blocks(const TailArgs& a);  // blocks of the backward pass
+int64_t tail_partial_floats(const TailArgs& a);  // size of `partial`; 0: the one block there is writes the gradients itself
 hipError_t launch_tail_forward(const TailArgs& a, bool normalize, hipStream_t s);
 hipError_t launch_tail_backward(const TailArgs& a, bool normalize, hipStream_t s);
 hipError_t launch_keep_mask(const TailArgs& a, uint8_t* out, hipStream_t s);

@@ -719,17 +719,26 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(Tail
       cols.store(y, k, d);
     }
   }
-  if (!a.partial) return;
-  float* out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * cols.width;
+  if (!a.grad_weight && !a.grad_bias) return;
+  // the block's sums of column c: to its part of `partial`, or (the only block) where they belong
+  float* const out = a.partial ? a.partial + static_cast<int64_t>(blockIdx.x) * 2 * cols.width : nullptr;
+  const auto give = [&](int c, float sw, float sb) {
+    if (out) {
+      out[c] = sw;
+      out[cols.width + c] = sb;
+    } else {
+      store_weight<T>(a.grad_weight, fp32, c, sw);
+      store_weight<T>(a.grad_bias, fp32, c, sb);
+    }
+  };
   if constexpr (W > 1) {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (cols.counts(k, j)) {
-          out[cols.at[k] + j] = IN_LDS ? mine[(k * (V / 4) + j / 4) * THREADS][j % 4] : dw[IN_LDS ? 0 : k][j];
-          out[cols.width + cols.at[k] + j] = IN_LDS ? mine[((K + k) * (V / 4) + j / 4) * THREADS][j % 4] : db[IN_LDS ? 0 : k][j];
-        }
+        if (cols.counts(k, j))
+          give(cols.at[k] + j, IN_LDS ? mine[(k * (V / 4) + j / 4) * THREADS][j % 4] : dw[IN_LDS ? 0 : k][j],
+               IN_LDS ? mine[((K + k) * (V / 4) + j / 4) * THREADS][j % 4] : db[IN_LDS ? 0 : k][j]);
     return;
   }
   // the teams of a wave, then the waves one after the other through LDS: a fixed order
@@ -756,10 +765,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(Tail
     }
     __syncthreads();
   }
-  for (int c = threadIdx.x; c < cols.width; c += THREADS) {
-    out[c] = columns[c];
-    out[cols.width + c] = columns[LANES * K * V + c];
-  }
+  for (int c = threadIdx.x; c < cols.width; c += THREADS) give(c, columns[c], columns[LANES * K * V + c]);
 }
 
 inline unsigned blocks_for(int64_t work, int64_t limit) { return static_cast<unsigned>(work < 1 ? 1 : work < limit ? work : limit); }
@@ -804,7 +810,8 @@ inline int64_t backward_blocks(const TailArgs& a, const Shape& h) {
   int64_t blocks = clamped(even((6 << 20) / (2 * block_bytes(a, h))), least, h.w < 8 ? 768 : 256);
   if (h.w > 1)  // a block's partial sums cost 8 bytes a feature each way: at least 16 rows a block
     blocks = clamped(even(a.rows / 16), 256, blocks);
-  return blocks_for(cdiv(a.rows, teams_in_block(h)), blocks);
+  const int64_t sweeps = cdiv(a.rows, teams_in_block(h));
+  return sweeps <= 4 ? 1 : blocks_for(sweeps, blocks);  // a few rows: one block, no partial sums and no second launch
 }
 
 template <class T, int G, int W, int K, bool SMOOTH>

@@ -81,6 +81,11 @@ int64_t tail_partial_blocks(const TailArgs& a) {
   const Shape h = shape_for(a.width, vec_of(a.dtype));
   return h.g ? backward_blocks(a, h) : blocks_for(a.rows, 256);
 }
+int64_t tail_partial_floats(const TailArgs& a) {
+  if (a.rows == 0) return 0;
+  const int64_t blocks = tail_partial_blocks(a);
+  return blocks == 1 && shape_for(a.width, vec_of(a.dtype)).g ? 0 : 2 * a.width * blocks;
+}
 
 hipError_t launch_tail_forward(const TailArgs& a, bool normalize, hipStream_t s) {
   switch (a.dtype) {
@@ -99,7 +104,7 @@ hipError_t launch_tail_backward(const TailArgs& a, bool normalize, hipStream_t s
     }
     if (e != hipSuccess) return e;
   }
-  if (a.grad_weight || a.grad_bias) {  // no rows: zeros
+  if ((a.grad_weight || a.grad_bias) && (a.partial || a.rows == 0)) {  // no rows: zeros
     if (a.width <= 256) launch_weight_gradient<4>(a, s);
     else if (a.width <= 1024) launch_weight_gradient<16>(a, s);
     else launch_weight_gradient<64>(a, s);

@@ -130,18 +130,17 @@ struct TailBackward : public torch::autograd::Node {
       const Rows g = rows_of(grad_y, width, !normalize);
       const bool need_w = task_should_compute_output(1), need_b = task_should_compute_output(2);
       if (task_should_compute_output(0)) out[0] = at::empty(grad_y.sizes(), grad_y.options());
-      Tensor workspace;
+      c10::DataPtr workspace;  // back to the allocator at the end of this block, in stream order like any tensor
       size_t bytes = 0;
       if (need_w) out[1] = at::empty({width}, grad_y.options().dtype(weight_type));
       if (need_b) out[2] = at::empty({width}, grad_y.options().dtype(weight_type));
       if (need_w || need_b) {
         bytes = g_lib.workspace_bytes(&desc, rows, width);
-        check(bytes ? 0 : AMBER_ERR_INVALID_ARGUMENT, "tail backward");
-        workspace = at::empty({static_cast<int64_t>(bytes)}, grad_y.options().dtype(at::kByte));
+        if (bytes) workspace = c10::GetAllocator(c10::DeviceType::CUDA)->allocate(bytes);
       }
       check(g_lib.backward(&desc, rows, width, data(xs), x_stride, data(g.t), g.stride, data(ws), static_cast<const float*>(data(ss)),
                            static_cast<const int64_t*>(data(st)), mutable_data(out[0]), mutable_data(out[1]), mutable_data(out[2]),
-                           mutable_data(workspace), bytes, stream_of(grad_y.device())),
+                           workspace.get(), bytes, stream_of(grad_y.device())),
             "tail backward");
     }
     if (at::GradMode::is_enabled()) {  // recorded (create_graph): allowed, but differentiating the gradients raises

@@ -411,6 +411,8 @@ int amber_mpn_estimate_num_elements(const int64_t* simplices, int32_t verts_per_
  * amber_mpn_tail_forward: x has row stride x_stride (elements; the features of a row are adjacent), y is dense.  stats:
  * float[2 rows] (mean, 1 / sqrt(var + eps) of every row) for the backward pass, or NULL.  Without `normalize` x must be dense.
  * amber_mpn_tail_backward: gradients from x, the forward's stats and grad_y (row stride g_stride; dense without `normalize`).
+ * workspace: amber_mpn_tail_backward_workspace_bytes (0 for few rows, without weights' gradients or for a description that the
+ * call itself will refuse), aligned to 4 bytes.
  * grad_x (dense), grad_weight, grad_bias: any may be NULL.  x may be NULL when neither normalize nor an activation needs it.
  * Sums over a row and over rows are in fp32 and in a fixed order: equal calls give equal bits.  Weights and their gradients are
  * of weight_dtype (fp32, or x's own type); weight / bias may each be NULL (1 and 0).

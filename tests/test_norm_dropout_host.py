@@ -92,14 +92,14 @@ def test_c_refusals_that_need_pointers_never_launch():
     assert lib.amber_mpn_tail_forward(plain, 4, 8, p, 8, p, 0, 0, p, 0, 0) == -1  # weight without normalize
     assert lib.amber_mpn_tail_forward(plain, 4, 8, p, 8, 0, p, 0, p, 0, 0) == -1
     back = lib.amber_mpn_tail_backward
-    need = lib.amber_mpn_tail_backward_workspace_bytes(d, 4, 8)
-    assert need >= 2 * 8 * 4
+    need = lib.amber_mpn_tail_backward_workspace_bytes(d, 4000, 8)
+    assert need >= 2 * 8 * 4 and lib.amber_mpn_tail_backward_workspace_bytes(d, 4, 8) == 0
     assert back(d, 4, 8, p, 8, 0, 8, 0, p, 0, p, 0, 0, 0, 0, 0) == -1  # grad_y
     assert back(d, 4, 8, 0, 8, p, 8, 0, p, 0, p, 0, 0, 0, 0, 0) == -1  # x
     assert back(d, 4, 8, p, 8, p, 8, 0, 0, 0, p, 0, 0, 0, 0, 0) == -1  # stats
     assert back(d, 4, 8, p, 8, p, -1, 0, p, 0, p, 0, 0, 0, 0, 0) == -1
-    assert back(d, 4, 8, p, 8, p, 8, 0, p, 0, p, p, 0, 0, 0, 0) == -1  # workspace
-    assert back(d, 4, 8, p, 8, p, 8, 0, p, 0, p, p, 0, p, need - 1, 0) == -3
+    assert back(d, 4000, 8, p, 8, p, 8, 0, p, 0, p, p, 0, 0, 0, 0) == -1  # workspace
+    assert back(d, 4000, 8, p, 8, p, 8, 0, p, 0, p, p, 0, p, need - 1, 0) == -3
     assert back(plain, 4, 8, 0, 8, p, 8, 0, 0, 0, p, 0, 0, 0, 0, 0) == -1  # the activation needs x
     assert back(plain, 4, 8, p, 8, p, 9, 0, 0, 0, p, 0, 0, 0, 0, 0) == -2
     assert back(plain, 4, 8, p, 8, p, 8, 0, 0, 0, p, p, 0, 0, 0, 0) == -1  # grad_weight without normalize
