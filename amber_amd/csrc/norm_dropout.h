@@ -90,7 +90,7 @@ DEVINL float tanh_of(float x) {
   p = fmaf(p, z, 0.13324906927244848f);
   p = fmaf(p, z, -0.3333307579068465f);
   p = fmaf(p, z, 0.99999998737373f);
-  const float far = 1.f - 2.f * rcp_of(1.f + exp_of(2.f * a));
+  const float far = fmaf(-2.f, rcp_of(1.f + exp_of(2.f * a)), 1.f);
   return a < 0.5f ? x * p : copysignf(far, x);
 }
 DEVINL float expm1_of(float x) {  // x <= 0
@@ -126,12 +126,12 @@ DEVINL float act_of(float x, int act) {
     case AMBER_ACT_ELU: return x > 0.f ? x : expm1_of(x);
     case AMBER_ACT_SILU: return x * rcp_of(1.f + exp_of(-x));
     case AMBER_ACT_MISH: {
-      const float w = exp_of(fminf(x, 20.f)), n = w * (w + 2.f);
+      const float w = exp_of(x > 20.f ? 20.f : x), n = w * (w + 2.f);
       return x * (n * rcp_of(n + 2.f));
     }
     case AMBER_ACT_GELU: {
       const float a = fabsf(x);
-      return fmaxf(x, 0.f) - fminf(a, 16.f) * gelu_parts(a).tail;
+      return fmaf(-fminf(a, 16.f), gelu_parts(a).tail, fmaxf(x, 0.f));
     }
     default: return x;
   }
@@ -153,13 +153,13 @@ DEVINL ActGrad act_grad(float x, int act) {
       return {x * s, s * fmaf(x, 1.f - s, 1.f)};
     }
     case AMBER_ACT_MISH: {
-      const float w = exp_of(fminf(x, 20.f)), n = w * (w + 2.f), r = rcp_of(n + 2.f), t = n * r;
-      return {x * t, fmaf(x * r, 4.f * w * (w + 1.f) * r, t)};
+      const float c = x > 20.f ? 20.f : x, w = exp_of(c), n = w * (w + 2.f), r = rcp_of(n + 2.f), t = n * r;
+      return {x * t, fmaf(c * r, 4.f * w * (w + 1.f) * r, t)};
     }
     case AMBER_ACT_GELU: {
       const float a = fabsf(x), ac = fminf(a, 16.f);
       const Gelu g = gelu_parts(a);
-      return {fmaxf(x, 0.f) - ac * g.tail, fmaf(copysignf(ac, x), 0.39894228040143268f * g.density, x < 0.f ? g.tail : 1.f - g.tail)};
+      return {fmaf(-ac, g.tail, fmaxf(x, 0.f)), fmaf(copysignf(ac, x), 0.39894228040143268f * g.density, x < 0.f ? g.tail : 1.f - g.tail)};
     }
     default: return {x, 1.f};
   }
@@ -197,10 +197,6 @@ DEVINL Words philox(const Stream& s, uint64_t group) {
   }
   return {{c0, c1, c2, c3}};
 }
-DEVINL bool kept(const TailArgs& a, const Stream& s, int64_t i) {
-  return philox(s, static_cast<uint64_t>(i) >> 2).w[i & 3] > a.last_dropped;
-}
-
 // v[j] of element first + j: 0 where dropped, else v[j] * scale.  A wave whose lanes all start at multiples of 4 takes V / 4 calls
 // of the generator, any other one more, its words moved down by first & 3.
 template <int V>
@@ -397,16 +393,20 @@ __global__ __launch_bounds__(kWide) void norm_forward_kernel(TailArgs a) {
     for (int c = threadIdx.x * V; c < width; c += kWide * V) {
       load(c);
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum[0] += c + j < width ? (v[j] - mean) * (v[j] - mean) : 0.f;
+      for (int j = 0; j < V; ++j) {
+        const float d = c + j < width ? v[j] - mean : 0.f;
+        sum[0] = fmaf(d, d, sum[0]);
+      }
     }
     sum[0] = team_sum<64>(sum[0]);
     join_waves<kWide / 64, 1>(sum, box[1]);
-    const float rstd = rsqrt_of(sum[0] * inv + a.eps);
+    const float rstd = rsqrt_of(fmaf(sum[0], inv, a.eps));
     for (int c = threadIdx.x * V; c < width; c += kWide * V) {
       load(c);
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (c + j < width) v[j] = (v[j] - mean) * rstd * load_weight<T>(a.weight, fp32, c + j, 1.f) + load_weight<T>(a.bias, fp32, c + j, 0.f);
+        if (c + j < width)
+          v[j] = fmaf((v[j] - mean) * rstd, load_weight<T>(a.weight, fp32, c + j, 1.f), load_weight<T>(a.bias, fp32, c + j, 0.f));
       if (a.drop) drop_pack(a, s, row * a.width + c, v);
       store_pack(y + c, width - c, v);
     }
@@ -448,12 +448,12 @@ __global__ __launch_bounds__(kWide) void norm_backward_kernel(TailArgs a) {
         if (pw) {  // a thread's own columns: nobody else touches them
           float* const at = pw + c + j;
           const bool first = row == blockIdx.x;
-          at[0] = first ? h[j] * n[j] : at[0] + h[j] * n[j];
+          at[0] = first ? h[j] * n[j] : fmaf(h[j], n[j], at[0]);
           at[width] = first ? h[j] : at[width] + h[j];
         }
         h[j] *= load_weight<T>(a.weight, fp32, c + j, 1.f);
         sums[0] += h[j];
-        sums[1] += h[j] * n[j];
+        sums[1] = fmaf(h[j], n[j], sums[1]);
       }
     }
     sums[0] = team_sum<64>(sums[0]);
@@ -466,7 +466,8 @@ __global__ __launch_bounds__(kWide) void norm_backward_kernel(TailArgs a) {
       load(c);
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (c + j < width) d[j] = rstd * (h[j] * load_weight<T>(a.weight, fp32, c + j, 1.f) - m0 - n[j] * m1) * d[j];
+        if (c + j < width)
+          d[j] = rstd * fmaf(-n[j], m1, fmaf(h[j], load_weight<T>(a.weight, fp32, c + j, 1.f), -m0)) * d[j];
       store_pack(y + c, width - c, d);
     }
   }
@@ -477,7 +478,8 @@ __global__ __launch_bounds__(kWide) void norm_backward_kernel(TailArgs a) {
 // ---------------------------------------------------------------------------------------------------
 // A lane's columns: pack k starts at (k LANES + lane) V, moved back to width - V where it would pass the row's end.  The lane then
 // holds columns that its neighbours hold too: they take no part in sums (element j of the last pack counts iff j >= skip) and are
-// stored twice with the same bits.  So every access is one full pack and no lane needs a path of its own.  NARROW (width < V, a
+// stored twice with the same bits (the compiler may not fuse multiplications and additions by itself here: it could do so for one
+// pack and not for another).  So every access is one full pack and no lane needs a path of its own.  NARROW (width < V, a
 // lane per row): element by element.
 template <class T, int LANES, int K, bool NARROW>
 struct Columns {
@@ -582,21 +584,24 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_forward(TailA
       for (int j = 0; j < V; ++j) v[k][j] -= mean;
       if (k < K - 1 || !ragged) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum[0] += v[k][j] * v[k][j];
+        for (int j = 0; j < V; ++j) sum[0] = fmaf(v[k][j], v[k][j], sum[0]);
       } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum[0] += cols.counts(k, j) ? v[k][j] * v[k][j] : 0.f;
+        for (int j = 0; j < V; ++j) {
+          const float c = cols.counts(k, j) ? v[k][j] : 0.f;
+          sum[0] = fmaf(c, c, sum[0]);
+        }
       }
     }
     sum[0] = team_sum<G>(sum[0]);
     join_waves<W, 1>(sum, box[1]);
-    const float rstd = rsqrt_of(sum[0] * inv + a.eps);
+    const float rstd = rsqrt_of(fmaf(sum[0], inv, a.eps));
     T* y = static_cast<T*>(a.y) + row * cols.width;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (k == K - 1 && !last) break;
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[k][j] = v[k][j] * rstd * w[k][j] + b[k][j];
+      for (int j = 0; j < V; ++j) v[k][j] = fmaf(v[k][j] * rstd, w[k][j], b[k][j]);
       if (a.drop) drop_pack(a, s, row * cols.width + cols.at[k], v[k]);
       cols.store(y, k, v[k]);
     }
@@ -673,7 +678,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(Tail
           Pack<float> tw = mine[(k * (V / 4) + q) * THREADS], tb = mine[((K + k) * (V / 4) + q) * THREADS];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            tw[j] += h[k][4 * q + j] * n[k][4 * q + j];
+            tw[j] = fmaf(h[k][4 * q + j], n[k][4 * q + j], tw[j]);
             tb[j] += h[k][4 * q + j];
           }
           mine[(k * (V / 4) + q) * THREADS] = tw;
@@ -682,7 +687,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(Tail
       } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          dw[IN_LDS ? 0 : k][j] += h[k][j] * n[k][j];
+          dw[IN_LDS ? 0 : k][j] = fmaf(h[k][j], n[k][j], dw[IN_LDS ? 0 : k][j]);
           db[IN_LDS ? 0 : k][j] += h[k][j];
         }
       }
@@ -692,14 +697,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(Tail
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           sums[0] += h[k][j];
-          sums[1] += h[k][j] * n[k][j];
+          sums[1] = fmaf(h[k][j], n[k][j], sums[1]);
         }
       } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float c = cols.counts(k, j) ? h[k][j] : 0.f;
           sums[0] += c;
-          sums[1] += c * n[k][j];
+          sums[1] = fmaf(c, n[k][j], sums[1]);
         }
       }
     }
@@ -715,7 +720,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(Tail
       if (k == K - 1 && !last) break;
       float d[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) d[j] = rstd * (h[k][j] - m0 - n[k][j] * m1) * dact[k][j];
+      for (int j = 0; j < V; ++j) d[j] = rstd * fmaf(-n[k][j], m1, h[k][j] - m0) * dact[k][j];
       cols.store(y, k, d);
     }
   }
@@ -816,7 +821,7 @@ inline int64_t backward_blocks(const TailArgs& a, const Shape& h) {
 
 template <class T, int G, int W, int K, bool SMOOTH>
 void launch_rows(const TailArgs& a, const Shape& h, bool backward, hipStream_t s) {
-    const dim3 block(W == 1 ? 256 : 64 * W);
+  const dim3 block(W == 1 ? 256 : 64 * W);
   if (backward)
     hipLaunchKernelGGL((norm_rows_backward<T, G, W, K, SMOOTH>), dim3(static_cast<unsigned>(backward_blocks(a, h))), block, 0, s, a);
   else

@@ -190,13 +190,19 @@ def broadcast_buffers(module: torch.nn.Module, src: int = 0, group=None) -> None
     (/root/reference/src/algorithm/core/amber.py:335); with graph-wise data parallelism one rank stays authoritative and
     the others take its numbers, so that every rank normalises its shard identically.  A no-op
     without an initialised process group or with one rank.  Device tensors under gloo are staged through the host (see
-    engine._sync_flat_gradient); RCCL takes them as they are."""
+    engine._sync_flat_gradient); RCCL takes them as they are.  A CounterGenerator's state stays the rank's own: ranks that see
+    different graphs draw different numbers."""
     import torch.distributed as dist
+
+    from .norm_dropout import CounterGenerator
 
     if not (dist.is_available() and dist.is_initialized()) or dist.get_world_size(group) == 1:
         return
     gloo = dist.get_backend(group) == "gloo"
+    own = {id(m.state) for m in module.modules() if isinstance(m, CounterGenerator)}
     for buf in module.buffers():
+        if id(buf) in own:
+            continue
         if buf.is_cuda and gloo:
             host = buf.detach().cpu()
             dist.broadcast(host, src=src, group=group)

@@ -216,6 +216,30 @@ def test_dropped_places_hold_zero_whatever_they_held(gpu_device):
     assert bool(torch.isnan(y[4]).all()) and bool(torch.isfinite(y[[0, 1, 2, 3, 5, 6, 7, 8]]).all())
 
 
+@pytest.mark.parametrize("act", ACTS)
+def test_activations_over_the_whole_range(gpu_device, act):
+    """Alone, in fp32, from -1e30 to 1e30 and NaN: value and derivative against float64.  The docstring's bounds (4 u |x| + 4 u |a|,
+    8 u (1 + |x|)) up to |x| = 90; beyond that every activation is 0, -1, 1 or x and its derivative 0 or 1."""
+    g = torch.Generator().manual_seed(6)
+    x = torch.cat([torch.linspace(-90, 90, 20001), torch.randn(20000, generator=g), torch.randn(20000, generator=g) * 1e-3,
+                   torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e-40, -1e-40, 0.5, -0.5, 20.0, 20.5, -20.0, 200.0, -200.0, 1e30, -1e30])])
+    xd = x.to(gpu_device).requires_grad_()
+    y = nd.activate_norm_dropout(xd, act, normalize=False)
+    dy, = torch.autograd.grad(y, xd, torch.ones_like(xd))
+    xr = x.double().requires_grad_()
+    want = orc.act(xr, act)
+    dwant, = torch.autograd.grad(want.sum(), xr)
+    far = xr.detach().abs().clamp(max=90)  # beyond: the value itself is exact, errors do not grow
+    err, derr = (y.detach().cpu().double() - want.detach()).abs(), (dy.cpu().double() - dwant).abs()
+    assert bool((err <= 4 * U * far + 5 * U * want.detach().abs() + 1e-37).all()), float((err / (far + 1e-30)).max() / U)
+    assert bool((derr <= 8 * U * (1 + far)).all()), float((derr / (1 + far)).max() / U)
+    odd = torch.tensor([float("nan"), float("inf")], device=gpu_device, requires_grad=True)
+    got = nd.activate_norm_dropout(odd, act, normalize=False)
+    grad, = torch.autograd.grad(got, odd, torch.ones_like(odd))
+    assert act in ("relu", "leakyrelu") or bool(torch.isnan(grad[0]))  # those two: a comparison, as torch's
+    assert bool(torch.isnan(got[0])) and float(got[1].detach()) == (1.0 if act == "tanh" else float("inf"))
+
+
 def test_constant_and_extreme_rows(gpu_device):
     w, b = torch.rand(100, device=gpu_device) + 0.5, torch.rand(100, device=gpu_device)
     for value in (0.0, 1.0, -3.75, 2.0 ** 60):  # sums of 100 equal powers-of-two multiples are exact: variance 0, y = bias
@@ -601,6 +625,16 @@ def test_training_step_with_the_counter_generator(gpu_device):
     assert torch.equal(work.edge_index.cpu(), g.edge_index.cpu()[:, kept]) and torch.equal(work.edge_attr.cpu(), g.edge_attr.cpu()[kept])
     with torch.no_grad():
         assert torch.equal(model.eval()(g), plain.eval()(g))
+
+
+@pytest.mark.parametrize("width", [6, 33, 130, 257, 333, 515, 777, 1027, 2049, 4099, 8190, 9001])
+def test_columns_held_twice_come_out_equal(gpu_device, width):
+    """Odd widths: two lanes hold and store some columns.  Whoever stores last, the bits are the same: twenty runs, forward and back."""
+    x, w, b, go = (t.to(gpu_device) for t in _data(400, width, torch.float32, torch.float32, seed=width))
+    state = _state(gpu_device)
+    first = _run(x, "tanh", w, b, True, 0.2, state, go)
+    for _ in range(20):
+        assert all(torch.equal(a, c) for a, c in zip(_run(x, "tanh", w, b, True, 0.2, state, go), first))
 
 
 def test_run_to_run_equality_under_load(gpu_device):

@@ -6,6 +6,7 @@ import math
 import numpy as np
 import pytest
 import torch
+import torch.multiprocessing as mp
 
 from amber_amd import _lib, norm_dropout as nd, synthetic as syn
 from amber_amd.architecture.mlp import MLP
@@ -210,3 +211,29 @@ def test_decoder_layers_without_a_generator_are_the_modules():
     for layer in mlp.mlp_layers:
         want = layer(want)
     assert torch.equal(mlp.run_layers(x), want)
+
+
+def _broadcast_worker(rank, port, ret):
+    import os
+
+    import torch.distributed as dist
+
+    from amber_amd import sharding
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    module = torch.nn.Sequential(torch.nn.BatchNorm1d(3), nd.CounterGenerator(40 + rank))
+    module[0].running_mean.fill_(float(rank + 1))
+    sharding.broadcast_buffers(module, src=0)
+    ret[rank] = (module[0].running_mean.tolist(), module[1].get_state())
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_world_size_2_broadcast_leaves_each_rank_its_generator():
+    import socket
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ret = mp.Manager().dict()
+    mp.spawn(_broadcast_worker, args=(port, ret), nprocs=2, join=True)
+    assert ret[0] == ([1.0] * 3, (40, 0)) and ret[1] == ([1.0] * 3, (41, 0))
