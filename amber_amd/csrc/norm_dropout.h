@@ -31,11 +31,22 @@ using Pack = T __attribute__((ext_vector_type(kVec<T>)));
 template <class T>
 using LoosePack = Pack<T> __attribute__((aligned(sizeof(T))));
 
+// Accesses past the caches (STREAM).  CACHE = 0: none.  1: the stores, where a call touches more than 1.5 times the 256 MB of the
+// memory-side cache: what it writes would not stay there for who reads it next, and would drive out what it still has to read
+// (32768 x 4096 bf16 dropout 102 -> 86 us).  2: the loads too, where the inputs alone do not fit (1.44 M x 128 fp32 LayerNorm
+// forward 250 -> 243 us, backward 409 -> 372, 6.0 TB/s).  Smaller calls are slower for it (5003 x 4099 bf16 backward 38 -> 46 us).
+template <bool STREAM, class T>
+DEVINL Pack<T> load_raw(const T* p) {
+  const LoosePack<T>* const q = reinterpret_cast<const LoosePack<T>*>(p);
+  if constexpr (STREAM) return __builtin_nontemporal_load(q);
+  else return *q;
+}
+
 // the first `count` of V elements (count >= V: all of them); the rest are 0
-template <class T, int V = kVec<T>>
+template <bool STREAM, class T, int V = kVec<T>>
 DEVINL void load_pack(const T* p, int count, float (&v)[V]) {
   if (count >= V) {
-    const Pack<T> q = *reinterpret_cast<const LoosePack<T>*>(p);
+    const Pack<T> q = load_raw<STREAM>(p);
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = to_f(q[j]);
   } else {
@@ -43,13 +54,15 @@ DEVINL void load_pack(const T* p, int count, float (&v)[V]) {
     for (int j = 0; j < V; ++j) v[j] = j < count ? to_f(p[j]) : 0.f;
   }
 }
-template <class T, int V = kVec<T>>
+template <bool STREAM, class T, int V = kVec<T>>
 DEVINL void store_pack(T* p, int count, const float (&v)[V]) {
   if (count >= V) {
     Pack<T> q;
 #pragma unroll
     for (int j = 0; j < V; ++j) q[j] = from_f<T>(v[j]);
-    *reinterpret_cast<LoosePack<T>*>(p) = q;
+    LoosePack<T>* const to = reinterpret_cast<LoosePack<T>*>(p);
+    if constexpr (STREAM) __builtin_nontemporal_store(q, to);
+    else *to = q;
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -274,7 +287,7 @@ DEVINL void act_any(int act, float (&v)[N], float (&d)[N]) {
 // ---------------------------------------------------------------------------------------------------
 // without the norm: elementwise over the flat tensor, 16 bytes a thread
 // ---------------------------------------------------------------------------------------------------
-template <class T, bool BWD, bool SMOOTH>
+template <class T, bool BWD, bool SMOOTH, int CACHE>
 __global__ __launch_bounds__(kBlock) void elementwise_kernel(TailArgs a) {
   constexpr int V = kVec<T>;
   Stream s{};
@@ -287,8 +300,8 @@ __global__ __launch_bounds__(kBlock) void elementwise_kernel(TailArgs a) {
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x) * V; i < n; i += step) {
     const int count = n - i < V ? static_cast<int>(n - i) : V;
     float v[V], xv[V];
-    if (BWD) load_pack(g + i, count, v);
-    if (!BWD || a.act != AMBER_ACT_NONE) load_pack(x + i, count, xv);
+    if (BWD) load_pack<CACHE == 2>(g + i, count, v);
+    if (!BWD || a.act != AMBER_ACT_NONE) load_pack<CACHE == 2>(x + i, count, xv);
     if (!BWD) {
       act_pack<SMOOTH, false>(a.act, xv, xv);
 #pragma unroll
@@ -301,7 +314,7 @@ __global__ __launch_bounds__(kBlock) void elementwise_kernel(TailArgs a) {
 #pragma unroll
       for (int j = 0; j < V; ++j) v[j] *= d[j];
     }
-    store_pack(y + i, count, v);
+    store_pack<CACHE >= 1>(y + i, count, v);
   }
 }
 
@@ -378,7 +391,7 @@ __global__ __launch_bounds__(kWide) void norm_forward_kernel(TailArgs a) {
     T* y = static_cast<T*>(a.y) + row * a.width;
     float sum[1] = {0.f}, v[V];
     const auto load = [&](int c) {
-      load_pack(x + c, width - c, v);
+      load_pack<false>(x + c, width - c, v);
       act_any<false>(a.act, v, v);  // 0 where the row has ended: act(0) = 0
     };
     for (int c = threadIdx.x * V; c < width; c += kWide * V) {
@@ -408,7 +421,7 @@ __global__ __launch_bounds__(kWide) void norm_forward_kernel(TailArgs a) {
         if (c + j < width)
           v[j] = fmaf((v[j] - mean) * rstd, load_weight<T>(a.weight, fp32, c + j, 1.f), load_weight<T>(a.bias, fp32, c + j, 0.f));
       if (a.drop) drop_pack(a, s, row * a.width + c, v);
-      store_pack(y + c, width - c, v);
+      store_pack<false>(y + c, width - c, v);
     }
     if (a.stats && threadIdx.x == 0) {
       a.stats[2 * row] = mean;
@@ -433,8 +446,8 @@ __global__ __launch_bounds__(kWide) void norm_backward_kernel(TailArgs a) {
     const float mean = a.stats[2 * row], rstd = a.stats[2 * row + 1];
     float sums[2] = {0.f, 0.f}, n[V], h[V], d[V];
     const auto load = [&](int c) {
-      load_pack(x + c, width - c, n);
-      load_pack(g + c, width - c, h);
+      load_pack<false>(x + c, width - c, n);
+      load_pack<false>(g + c, width - c, h);
       act_any<true>(a.act, n, d);
       if (a.drop) drop_pack(a, s, row * a.width + c, h);
 #pragma unroll
@@ -468,7 +481,7 @@ __global__ __launch_bounds__(kWide) void norm_backward_kernel(TailArgs a) {
       for (int j = 0; j < V; ++j)
         if (c + j < width)
           d[j] = rstd * fmaf(-n[j], m1, fmaf(h[j], load_weight<T>(a.weight, fp32, c + j, 1.f), -m0)) * d[j];
-      store_pack(y + c, width - c, d);
+      store_pack<false>(y + c, width - c, d);
     }
   }
 }
@@ -481,7 +494,7 @@ __global__ __launch_bounds__(kWide) void norm_backward_kernel(TailArgs a) {
 // stored twice with the same bits (the compiler may not fuse multiplications and additions by itself here: it could do so for one
 // pack and not for another).  So every access is one full pack and no lane needs a path of its own.  NARROW (width < V, a
 // lane per row): element by element.
-template <class T, int LANES, int K, bool NARROW>
+template <class T, int LANES, int K, bool NARROW, int CACHE>
 struct Columns {
   static constexpr int V = kVec<T>;
   using Raw = Pack<T>;
@@ -501,13 +514,13 @@ struct Columns {
 #pragma unroll
         for (int j = 0; j < V; ++j) raw[k][j] = j < width ? row[j] : from_f<T>(0.f);
       } else {
-        raw[k] = *reinterpret_cast<const LoosePack<T>*>(row + at[k]);
+        raw[k] = load_raw<CACHE == 2>(row + at[k]);
       }
     }
   }
   DEVINL void store(T* row, int k, const float (&v)[V]) const {
     if (!stores(k)) return;
-    store_pack(row + at[k], NARROW ? width : V, v);
+    store_pack<CACHE >= 1>(row + at[k], NARROW ? width : V, v);
   }
   // weight or bias of pack k in fp32
   DEVINL void load_weight_pack(const void* w, bool fp32, float missing, int k, float (&v)[V]) const {
@@ -535,12 +548,12 @@ struct Columns {
 
 // One row per team and sweep; the next sweep's loads are issued before this one's arithmetic.  (Two rows a sweep, or four, were
 // slower: 1.44 M x 128 fp32 forward 292 us instead of 250.)
-template <class T, int G, int W, int K, bool SMOOTH>
+template <class T, int G, int W, int K, bool SMOOTH, int CACHE>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_forward(TailArgs a) {
   constexpr int V = kVec<T>, LANES = G * W, THREADS = W == 1 ? 256 : 64 * W, TEAMS = THREADS / LANES;
   __shared__ float box[2][W][1];
   const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
-  const Columns<T, LANES, K, LANES == 1> cols(lane, static_cast<int>(a.width));
+  const Columns<T, LANES, K, LANES == 1, CACHE> cols(lane, static_cast<int>(a.width));
   const bool ragged = cols.ragged(), last = W == 1 || __any(cols.stores(K - 1));  // a wave without columns in the last pack skips it
   const float width = static_cast<float>(cols.width), inv = 1.f / width;
   const T* x = static_cast<const T*>(a.x);
@@ -615,7 +628,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_forward(TailA
 // Needs x, the gradient and two statistics of a row; the gradients of weight and bias gather over a team's rows, in registers (W = 16,
 // rows beyond 8192 features: 128 registers a lane are too few, so in LDS, where every thread adds to places of its own), and are
 // joined over the block at its end.  Two rows on their way instead of one changed nothing (20000 x 8192 fp32 381 us, 385).
-template <class T, int G, int W, int K, bool SMOOTH>
+template <class T, int G, int W, int K, bool SMOOTH, int CACHE>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(TailArgs a) {
   constexpr int V = kVec<T>, LANES = G * W, THREADS = W == 1 ? 256 : 64 * W, TEAMS = THREADS / LANES;
   constexpr bool IN_LDS = W == 16, AHEAD = !(IN_LDS && K * V == 16);
@@ -624,7 +637,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(Tail
   __shared__ __attribute__((aligned(16))) float columns[W == 1 || IN_LDS ? 2 * LANES * K * V : 4];
   Pack<float>* const mine = reinterpret_cast<Pack<float>*>(columns) + threadIdx.x;
   const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
-  const Columns<T, LANES, K, LANES == 1> cols(lane, static_cast<int>(a.width));
+  const Columns<T, LANES, K, LANES == 1, CACHE> cols(lane, static_cast<int>(a.width));
   const bool ragged = cols.ragged(), last = W == 1 || __any(cols.stores(K - 1)), fp32 = a.weight_dtype == AMBER_DTYPE_F32;
   const float inv = 1.f / static_cast<float>(cols.width);
   const T* x = static_cast<const T*>(a.x);
@@ -819,18 +832,23 @@ inline int64_t backward_blocks(const TailArgs& a, const Shape& h) {
   return sweeps <= 4 ? 1 : blocks_for(sweeps, blocks);  // a few rows: one block, no partial sums and no second launch
 }
 
-template <class T, int G, int W, int K, bool SMOOTH>
+inline int cache_mode(const TailArgs& a, int inputs) {
+  const int64_t bytes = a.rows * a.width * (16 / vec_of(a.dtype));
+  return inputs * bytes > 300000000 ? 2 : (inputs + 1) * bytes > 384000000 ? 1 : 0;
+}
+
+template <class T, int G, int W, int K, bool SMOOTH, int CACHE>
 void launch_rows(const TailArgs& a, const Shape& h, bool backward, hipStream_t s) {
   const dim3 block(W == 1 ? 256 : 64 * W);
   if (backward)
-    hipLaunchKernelGGL((norm_rows_backward<T, G, W, K, SMOOTH>), dim3(static_cast<unsigned>(backward_blocks(a, h))), block, 0, s, a);
+    hipLaunchKernelGGL((norm_rows_backward<T, G, W, K, SMOOTH, CACHE>), dim3(static_cast<unsigned>(backward_blocks(a, h))), block, 0, s, a);
   else
-    hipLaunchKernelGGL((norm_rows_forward<T, G, W, K, SMOOTH>), dim3(static_cast<unsigned>(forward_blocks(a, h))), block, 0, s, a);
+    hipLaunchKernelGGL((norm_rows_forward<T, G, W, K, SMOOTH, CACHE>), dim3(static_cast<unsigned>(forward_blocks(a, h))), block, 0, s, a);
 }
-template <class T, bool SMOOTH>
+template <class T, bool SMOOTH, int CACHE>
 void launch_shape(const TailArgs& a, const Shape& h, bool backward, hipStream_t s) {
 #define AMBER_ROWS(G, W, K) \
-  if (h.g == G && h.w == W && h.k == K) return launch_rows<T, G, W, K, SMOOTH>(a, h, backward, s)
+  if (h.g == G && h.w == W && h.k == K) return launch_rows<T, G, W, K, SMOOTH, CACHE>(a, h, backward, s)
   AMBER_ROWS(1, 1, 1);
   AMBER_ROWS(2, 1, 1);
   AMBER_ROWS(4, 1, 1);
@@ -857,37 +875,43 @@ void launch_shape(const TailArgs& a, const Shape& h, bool backward, hipStream_t 
   }
 #undef AMBER_ROWS
 }
-template <class T, bool BWD>
+template <class T, bool BWD, bool SMOOTH>
 void launch_elementwise(const TailArgs& a, hipStream_t s) {
   const dim3 grid(blocks_for(cdiv(a.rows * a.width, kBlock * kVec<T>), kMaxBlocks));
-  if (is_smooth(a.act))
-    hipLaunchKernelGGL((elementwise_kernel<T, BWD, true>), grid, dim3(kBlock), 0, s, a);
-  else
-    hipLaunchKernelGGL((elementwise_kernel<T, BWD, false>), grid, dim3(kBlock), 0, s, a);
+  switch (cache_mode(a, BWD && a.act != AMBER_ACT_NONE ? 2 : 1)) {
+    case 0: hipLaunchKernelGGL((elementwise_kernel<T, BWD, SMOOTH, 0>), grid, dim3(kBlock), 0, s, a); break;
+    case 1: hipLaunchKernelGGL((elementwise_kernel<T, BWD, SMOOTH, 1>), grid, dim3(kBlock), 0, s, a); break;
+    default: hipLaunchKernelGGL((elementwise_kernel<T, BWD, SMOOTH, 2>), grid, dim3(kBlock), 0, s, a);
+  }
 }
-template <class T>
+template <class T, bool SMOOTH>
 bool launch_in_registers(const TailArgs& a, bool backward, hipStream_t s) {
   const Shape h = shape_for(a.width, kVec<T>);
   if (h.g == 0) return false;
-  if (is_smooth(a.act)) launch_shape<T, true>(a, h, backward, s);
-  else launch_shape<T, false>(a, h, backward, s);
+  switch (cache_mode(a, backward ? 2 : 1)) {
+    case 0: launch_shape<T, SMOOTH, 0>(a, h, backward, s); break;
+    case 1: launch_shape<T, SMOOTH, 1>(a, h, backward, s); break;
+    default: launch_shape<T, SMOOTH, 2>(a, h, backward, s);
+  }
   return true;
 }
 
 template <class T>
 hipError_t tail_forward_t(const TailArgs& a, bool normalize, hipStream_t s) {
+  const bool smooth = is_smooth(a.act);
   if (!normalize)
-    launch_elementwise<T, false>(a, s);
-  else if (!launch_in_registers<T>(a, false, s))
+    smooth ? launch_elementwise<T, false, true>(a, s) : launch_elementwise<T, false, false>(a, s);
+  else if (!(smooth ? launch_in_registers<T, true>(a, false, s) : launch_in_registers<T, false>(a, false, s)))
     hipLaunchKernelGGL((norm_forward_kernel<T>), dim3(blocks_for(a.rows, 512)), dim3(kWide), 0, s, a);
   return hipGetLastError();
 }
 // dx and, into a.partial, the blocks' sums for the weights' gradients
 template <class T>
 hipError_t tail_backward_t(const TailArgs& a, bool normalize, hipStream_t s) {
+  const bool smooth = is_smooth(a.act);
   if (!normalize)
-    launch_elementwise<T, true>(a, s);
-  else if (!launch_in_registers<T>(a, true, s))
+    smooth ? launch_elementwise<T, true, true>(a, s) : launch_elementwise<T, true, false>(a, s);
+  else if (!(smooth ? launch_in_registers<T, true>(a, true, s) : launch_in_registers<T, false>(a, true, s)))
     hipLaunchKernelGGL((norm_backward_kernel<T>), dim3(static_cast<unsigned>(tail_partial_blocks(a))), dim3(kWide), 0, s, a);
   return hipGetLastError();
 }
