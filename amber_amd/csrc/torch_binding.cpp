@@ -65,7 +65,8 @@ void check_probability(double p) {
   TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "Dropout probability has to be between 0 and 1 (got ", p, ")");
 }
 void check_sequence(int64_t sequence) {
-  TORCH_CHECK_VALUE(sequence >= 0 && sequence < (int64_t{1} << 62), "amber_amd: sequence has to be between 0 and 2**62 (got ", sequence, ")");
+  TORCH_CHECK_VALUE(sequence >= 0 && sequence < (int64_t{1} << 62), "amber_amd: sequence has to be between 0 and 2**62 (got ", sequence,
+                    ")");
 }
 void check_state(const std::optional<Tensor>& state) {
   TORCH_CHECK_VALUE(state.has_value() && state->defined(), "amber_amd: dropout needs the generator's `state` (CounterGenerator.take())");
@@ -102,11 +103,21 @@ void* mutable_data(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() 
 
 struct TailBackward : public torch::autograd::Node {
   AmberTailDesc desc{};
-  int64_t x_stride = 0;
   at::ScalarType weight_type = at::kFloat;
   SavedVariable x, weight, stats, state;
 
   std::string name() const override { return "AmberTailBackward"; }
+
+  // What was saved may come back from a saved tensors' hook with other strides (a copy that was on the host, say): its layout is
+  // looked at here, not remembered.
+  static Rows saved(const Tensor& from, const char* name, int64_t rows, int64_t width, at::ScalarType type, const at::Device& device,
+                    bool dense) {
+    if (!from.defined()) return {from, width};
+    TORCH_CHECK(from.numel() == rows * width && (dense || from.size(-1) == width) && from.scalar_type() == type && from.device() == device,
+                "amber_amd: `", name, "` was saved for the backward pass and came back as another tensor: ", from.scalar_type(), " ",
+                from.sizes(), " on ", from.device());
+    return rows_of(plain(from), width, dense);
+  }
 
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -127,7 +138,10 @@ struct TailBackward : public torch::autograd::Node {
       const Tensor grad_y = plain(grads[0]);
       const bool normalize = desc.normalize != 0;
       const int64_t width = normalize ? grad_y.size(-1) : 1, rows = grad_y.numel() / width;
-      const Rows g = rows_of(grad_y, width, !normalize);
+      const Rows g = rows_of(grad_y, width, !normalize), r = saved(xs, "x", rows, width, grad_y.scalar_type(), grad_y.device(), !normalize),
+                 w = saved(ws, "weight", 1, width, weight_type, grad_y.device(), true),
+                 s = saved(ss, "stats", 2, rows, at::kFloat, grad_y.device(), true),
+                 t = saved(st, "state", 1, 2, at::kLong, grad_y.device(), true);
       const bool need_w = task_should_compute_output(1), need_b = task_should_compute_output(2);
       if (task_should_compute_output(0)) out[0] = at::empty(grad_y.sizes(), grad_y.options());
       c10::DataPtr workspace;  // back to the allocator at the end of this block, in stream order like any tensor
@@ -138,8 +152,8 @@ struct TailBackward : public torch::autograd::Node {
         bytes = g_lib.workspace_bytes(&desc, rows, width);
         if (bytes) workspace = c10::GetAllocator(c10::DeviceType::CUDA)->allocate(bytes);
       }
-      check(g_lib.backward(&desc, rows, width, data(xs), x_stride, data(g.t), g.stride, data(ws), static_cast<const float*>(data(ss)),
-                           static_cast<const int64_t*>(data(st)), mutable_data(out[0]), mutable_data(out[1]), mutable_data(out[2]),
+      check(g_lib.backward(&desc, rows, width, data(r.t), r.stride, data(g.t), g.stride, data(w.t), static_cast<const float*>(data(s.t)),
+                           static_cast<const int64_t*>(data(t.t)), mutable_data(out[0]), mutable_data(out[1]), mutable_data(out[2]),
                            workspace.get(), bytes, stream_of(grad_y.device())),
             "tail backward");
     }
@@ -218,15 +232,14 @@ Tensor tail(const Tensor& x_, const std::optional<Tensor>& weight_, const std::o
     const Tensor b = bias.defined() ? bias.contiguous() : bias;
     y = at::empty(x.sizes(), x.options());
     if (normalize && record) stats = at::empty({2 * rows}, x.options().dtype(at::kFloat));
-    check(g_lib.forward(&desc, rows, width, data(r.t), r.stride, data(w), data(b), static_cast<const int64_t*>(data(state)), mutable_data(y),
-                        static_cast<float*>(mutable_data(stats)), stream_of(x.device())),
+    check(g_lib.forward(&desc, rows, width, data(r.t), r.stride, data(w), data(b), static_cast<const int64_t*>(data(state)),
+                        mutable_data(y), static_cast<float*>(mutable_data(stats)), stream_of(x.device())),
           "tail forward");
   }
   if (record) {
     std::shared_ptr<TailBackward> node(new TailBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(x, weight, bias));
     node->desc = desc;
-    node->x_stride = r.stride;
     node->weight_type = weight_type;
     // x itself where the kernels read it in place: a change of it before the backward pass is noticed
     if (normalize || activation != AMBER_ACT_NONE)
@@ -259,8 +272,10 @@ Tensor generator_take(const Tensor& state, int64_t count) {
   check_device(state, "generator state");
   const c10::DeviceGuard guard(state.device());
   const Tensor taken = at::empty_like(state);
-  state.unsafeGetTensorImpl()->bump_version();  // a backward pass that reads the generator's own buffer instead of `taken` must notice
-  check(g_lib.take(state.mutable_data_ptr<int64_t>(), count, taken.mutable_data_ptr<int64_t>(), stream_of(state.device())), "generator take");
+  // a backward pass that reads the generator's own buffer instead of `taken` must notice
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+  check(g_lib.take(state.mutable_data_ptr<int64_t>(), count, taken.mutable_data_ptr<int64_t>(), stream_of(state.device())),
+        "generator take");
   return taken;
 }
 

@@ -19,6 +19,9 @@ anything else is copied first.  First derivatives only.
 Inside a HIP graph: `take` and the operators may be captured; the generator's state lives on the device, so every replay draws
 new numbers.  Capturing a backward pass follows torch's own rule: no autograd graph that was recorded outside the capture may
 still hold the same leaves.
+
+Recomputing (torch.utils.checkpoint): call `take` outside the recomputed function and hand its result in; a `take` that is run
+again draws other numbers.
 """
 from __future__ import annotations
 

@@ -16,6 +16,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from amber_amd import norm_dropout as nd, synthetic as syn
 from amber_amd.architecture.mlp import MLP
@@ -446,6 +447,69 @@ def test_generator_buffer_as_state_is_guarded(gpu_device):
         y.sum().backward()
 
 
+@pytest.mark.parametrize("shape", [(60, 64), (5, 12, 64)])
+def test_saved_tensors_may_move(gpu_device, shape):
+    """x, weight, statistics and state go through the host and come back contiguous, whatever rows x had in the forward pass; x alone
+    comes back with rows further apart; a hook that changes the type is refused."""
+    base = torch.randn(*shape[:-1], 130, device=gpu_device)
+    w, b = torch.randn(64, device=gpu_device), torch.randn(64, device=gpu_device)
+    state, go = nd.CounterGenerator(3, gpu_device).take(), torch.randn(shape, device=gpu_device)
+
+    def gradients(x, hooks):
+        leaves = [t.detach().clone().requires_grad_() for t in (w, b)]
+        xl = x.detach().requires_grad_()
+        with hooks:
+            y = nd.activate_norm_dropout(xl, "silu", *leaves, p=0.25, state=state)
+            z = nd.activate_norm_dropout(y, "mish", normalize=False, p=0.25, state=state, sequence=1)
+        return torch.autograd.grad(z, [xl, *leaves], go)
+
+    def keep(t):
+        return t
+
+    def spread(t):
+        if t.dim() < 2:
+            return t
+        wide = t.new_full((*t.shape[:-1], t.shape[-1] + 7), float("nan"))
+        wide[..., :t.shape[-1]] = t
+        return wide[..., :t.shape[-1]]
+
+    for x in (base[..., :64], base[..., 3:67], base[..., :64].contiguous()):
+        want = gradients(x, torch.autograd.graph.saved_tensors_hooks(keep, keep))
+        for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(keep, spread)):
+            for a, b_ in zip(want, gradients(x, hooks)):
+                assert torch.equal(a, b_)
+    with pytest.raises(RuntimeError, match="came back as another tensor"):
+        gradients(base[..., :64], torch.autograd.graph.saved_tensors_hooks(keep, lambda t: t.double()))
+
+
+def test_recomputed_layers(gpu_device):
+    """torch.utils.checkpoint with the range taken outside gives the gradients of the plain call."""
+    x, state = torch.randn(50, 70, device=gpu_device), nd.CounterGenerator(4, gpu_device).take()
+    w = torch.randn(70, device=gpu_device, requires_grad=True)
+    want = None
+    for reentrant in (None, False, True):
+        xl = x.clone().requires_grad_()
+        f = lambda t: nd.activate_norm_dropout(t * 2, "elu", w, p=0.3, state=state)
+        y = f(xl) if reentrant is None else torch.utils.checkpoint.checkpoint(f, xl, use_reentrant=reentrant)
+        w.grad = None
+        y.square().sum().backward()
+        got = (y.detach(), xl.grad, w.grad)
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_inference_mode(gpu_device):
+    x = torch.randn(9, 33, device=gpu_device)
+    with torch.inference_mode():
+        gen = nd.CounterGenerator(8, gpu_device)
+        a = nd.activate_norm_dropout(x, "relu", p=0.5, state=gen.take())
+    outside = nd.CounterGenerator(8, gpu_device)
+    assert torch.equal(a, nd.activate_norm_dropout(x, "relu", p=0.5, state=outside.take()))
+    with torch.inference_mode():
+        gen.take(), outside.take()
+        assert gen.get_state() == outside.get_state() == (8, 2)
+
+
 def test_forward_mode_is_refused(gpu_device):
     import torch.autograd.forward_ad as fwd
     x = torch.randn(4, 8, device=gpu_device)
@@ -552,6 +616,47 @@ def test_captured_step_draws_anew_at_every_replay(gpu_device):
     torch.cuda.synchronize()
     assert gen.get_state() == (4242, 110)
     assert all(not torch.equal(out[0], t) for t in seen)
+
+
+def test_two_graphs_of_one_generator(gpu_device):
+    """Steps of two sizes, captured one by one from one generator and replayed in turn with eager steps between them: each draws the
+    generator's next range, and neither disturbs the other's workspace."""
+    gen, graphs = nd.CounterGenerator(77, device=gpu_device), []
+    sizes = ((900, 96), (70, 1030))
+    data = [tuple(t.to(gpu_device) for t in _data(*size, torch.float32, torch.float32, seed=13 + i)) for i, size in enumerate(sizes)]
+
+    def step(x, w, b, go):
+        state = gen.take()
+        xr, wr, br = (t.detach().requires_grad_() for t in (x, w, b))
+        y = nd.activate_norm_dropout(xr, "leakyrelu", wr, br, p=0.2, state=state)
+        return (y.detach(),) + torch.autograd.grad(y, (xr, wr, br), go)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for d in data:
+            step(*d)
+    torch.cuda.current_stream().wait_stream(side)
+    for d in data:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*d)
+        graphs.append((graph, out))
+    gen.set_state(77, 0)
+    got = []
+    for which in (0, 1, 1, 0, 2, 0, 1):  # 2: an eager step
+        if which == 2:
+            step(*data[0])
+            got.append(None)
+            continue
+        graphs[which][0].replay()
+        got.append((which, [t.clone() for t in graphs[which][1]]))
+    torch.cuda.synchronize()
+    assert gen.get_state() == (77, len(got))
+    gen.set_state(77, 0)
+    for entry in got:
+        want = step(*data[entry[0] if entry else 0])
+        assert entry is None or all(torch.equal(a, c) for a, c in zip(entry[1], want))
 
 
 def _decoder(norm, p, act, layers=2, latent=64):
