@@ -570,7 +570,7 @@ struct Columns {
 };
 
 // One row per team and sweep; the next sweep's loads are issued before this one's arithmetic.  (Two rows a sweep, or four, were
-// slower: 1.44 M x 128 fp32 forward 292 us instead of 250.)
+// slower: 1.44 M x 128 fp32 forward 292 us instead of 250, cached.)
 template <class T, int G, int W, int K, bool SMOOTH, int CACHE>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_forward(TailArgs a) {
   constexpr int V = kVec<T>, LANES = G * W, THREADS = W == 1 ? 256 : 64 * W, TEAMS = THREADS / LANES;
@@ -832,7 +832,8 @@ inline Shape shape_for(int64_t width, int vec) {
 inline int64_t teams_in_block(const Shape& h) { return h.w > 1 ? 1 : 256 / h.g; }
 // Blocks of a launch: each takes rows in turn and has the next ones on their way, so their number sets the bytes in flight.  About
 // 4 MB forward and 6 MB backward (x and the gradient) are best; more only spread the accesses over more pages: 1.44 M x 128 fp32
-// forward 250 us with 1024 blocks (5.9 TB/s), 311 with 512, 328 with 2048; 100000 x 1024 fp32 backward 219 with 256, 237 with 1024.
+// forward 250 us with 1024 blocks, 311 with 512, 328 with 2048 (before its accesses went past the caches: 244 us now, 6.0 TB/s);
+// 100000 x 1024 fp32 backward 219 with 256, 237 with 1024.
 // The generator and the smooth activations ask for more waves than that: 100000 x 2048 bf16 forward with dropout 292 us with 512
 // blocks, 185 with 1280; 100000 x 1024 fp32 184 with 256, 154 with 768.  Measured from 32 to 16384 features, 1000 to 2 M rows, fp32
 // and bf16, with and without dropout, in steps of 256 blocks: a CU more or less than the others counts (100000 x 1020 fp32 forward
