@@ -552,6 +552,38 @@ def test_offsets_beyond_32_bits(gpu_device):
     assert torch.equal(mask[-9:].cpu(), orc.keep(9, 0.3, 1234567890123, 17, start=1 << 32))
 
 
+@pytest.mark.parametrize("megabytes", [150, 220, 330])
+@pytest.mark.parametrize("width, dtype", [(128, "fp32"), (1021, "fp32"), (333, "fp16"), (4099, "bf16"), (16400, "bf16")])
+def test_large_calls_give_the_small_calls_rows(gpu_device, width, dtype, megabytes):
+    """Tensors around what the caches hold: every row of a large call has the bits of the same row in a call of a few rows, and the
+    dropped places are the mask's."""
+    t = DTYPES[dtype]
+    rows = megabytes * 10 ** 6 // (width * t.itemsize) + 1
+    torch.manual_seed(width + megabytes)
+    x, g = (torch.randn(rows, width, device=gpu_device, dtype=t) for _ in range(2))
+    w, b, state = torch.randn(width, device=gpu_device), torch.randn(width, device=gpu_device), _state(gpu_device)
+
+    def both(x, g, **kw):
+        xr = x.detach().requires_grad_()
+        y = nd.activate_norm_dropout(xr, "leakyrelu", **kw)
+        return y.detach(), torch.autograd.grad(y, xr, g)[0]
+
+    for kw in (dict(weight=w, bias=b), dict(normalize=False)):
+        large = both(x, g, **kw)
+        for first in (0, rows // 2, rows - 7):
+            small = both(x[first:first + 7], g[first:first + 7], **kw)
+            assert all(torch.equal(a[first:first + 7], c) for a, c in zip(large, small))
+        for part in torch.arange(rows, device=gpu_device).split(rows // 9 + 1):  # all rows, a ninth at a time
+            small = both(x[part[0]:part[-1] + 1], g[part[0]:part[-1] + 1], **kw)
+            assert all(torch.equal(a[part[0]:part[-1] + 1], c) for a, c in zip(large, small))
+    keep = nd.keep_mask(x.numel(), 0.25, state).view(x.shape)
+    y, dx = both(x, g, normalize=False, p=0.25, state=state)
+    scale = torch.tensor(1 / 0.75, dtype=torch.float32, device=gpu_device)
+    slope = torch.where(x > 0, 1.0, torch.tensor(0.01, device=gpu_device))
+    assert torch.equal(y, torch.where(keep, x.float() * slope * scale, 0.0).to(t))
+    assert torch.equal(dx, torch.where(keep, g.float() * scale * slope, 0.0).to(t))
+
+
 def test_other_stream_and_two_at_once(gpu_device):
     x, w, b, go = (t.to(gpu_device) for t in _data(3000, 200, torch.float32, torch.float32, seed=9))
     state = _state(gpu_device)
