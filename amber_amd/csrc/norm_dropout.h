@@ -850,9 +850,11 @@ inline int64_t backward_blocks(const TailArgs& a, const Shape& h) {
   const bool half = a.dtype != AMBER_DTYPE_F32;
   const int64_t least = a.drop && half && h.w < 8 ? 512 : 256;
   int64_t blocks = clamped(even((6 << 20) / (2 * block_bytes(a, h))), least, h.w < 8 ? 768 : 256);
-  if (h.w > 1)  // a block's partial sums cost 8 bytes a feature each way: at least 16 rows a block
-    blocks = clamped(even(a.rows / 16), 256, blocks);
   const int64_t sweeps = cdiv(a.rows, teams_in_block(h));
+  // A block's partial sums cost 8 bytes a feature each way, and its join some microseconds: at least 3 sweeps a block (6000 x 256 bf16
+  // 10.3 us with 256 blocks, 12.1 with 750; 2000 x 1021 13.0 and 16.7 with 500), 16 rows where a block takes one row at a time (5003 x
+  // 4096 bf16 33 us with 256, 35 with 512), 12 of one pack a lane (5003 x 1500 bf16 20.8 with 512, 24.7 with 256).
+  blocks = clamped(even(sweeps / (h.w == 1 ? 3 : h.k == 1 ? 12 : 16)), 256, blocks);
   return sweeps <= 4 ? 1 : blocks_for(sweeps, blocks);  // a few rows: one block, no partial sums and no second launch
 }
 
