@@ -210,10 +210,10 @@ DEVINL Words philox(const Stream& s, uint64_t group) {
   }
   return {{c0, c1, c2, c3}};
 }
-// v[j] of element first + j: 0 where dropped, else v[j] * scale.  A wave whose lanes all start at multiples of 4 takes V / 4 calls
-// of the generator, any other one more, its words moved down by first & 3.
-template <int V>
-DEVINL void drop_pack(const TailArgs& a, const Stream& s, int64_t first, float (&v)[V]) {
+// v[j] of element first + j: +0 where dropped, else kept(j).  A wave whose lanes all start at multiples of 4 takes V / 4 calls of the
+// generator, any other one more, its words moved down by first & 3.
+template <int V, class Kept>
+DEVINL void select_pack(const TailArgs& a, const Stream& s, int64_t first, float (&v)[V], const Kept& kept) {
   uint32_t w[V + 4];
   const uint64_t group = static_cast<uint64_t>(first) >> 2;
 #pragma unroll
@@ -241,7 +241,11 @@ DEVINL void drop_pack(const TailArgs& a, const Stream& s, int64_t first, float (
     }
   }
 #pragma unroll
-  for (int j = 0; j < V; ++j) v[j] = w[j] > a.last_dropped ? v[j] * a.scale : 0.f;
+  for (int j = 0; j < V; ++j) v[j] = w[j] > a.last_dropped ? kept(j) : 0.f;
+}
+template <int V>
+DEVINL void drop_pack(const TailArgs& a, const Stream& s, int64_t first, float (&v)[V]) {
+  select_pack(a, s, first, v, [&](int j) { return v[j] * a.scale; });
 }
 
 // v = act(v), d = act'(v) (if wanted) on N values: the choice is uniform and made outside the loops.  SMOOTH: the activations beyond
@@ -309,12 +313,17 @@ __global__ __launch_bounds__(kBlock) void elementwise_kernel(TailArgs a) {
   // v = what the dropout applies to, z = the pre-activation
   const auto work = [&](float (&v)[V], float (&z)[V], int64_t first) {
     if (!BWD) act_pack<SMOOTH, false>(a.act, v, v);
-    if (a.drop) drop_pack(a, s, first, v);
     if (BWD && a.act != AMBER_ACT_NONE) {
       float d[V];
       act_pack<SMOOTH, true>(a.act, z, d);
+      if (a.drop) {  // selected last: the derivative may be negative (-0), NaN or infinite where the gradient is 0
+        select_pack(a, s, first, v, [&](int j) { return v[j] * a.scale * d[j]; });
+      } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] *= d[j];
+        for (int j = 0; j < V; ++j) v[j] *= d[j];
+      }
+    } else if (a.drop) {
+      drop_pack(a, s, first, v);
     }
   };
   for (; p < packs; p += step) {

@@ -10,7 +10,8 @@ there is no CPU path.
     keep = keep_mask(num_edges, 0.1, state)
 
 Element i (row-major) of a call owns word i & 3 of Philox-4x32-10 under key `seed` at counter (i >> 2, offset + sequence); it is
-dropped iff the word is below floor(p 2^32).  A dropped element is +0 whatever it held, and so is its gradient.
+dropped iff the word is below floor(p 2^32).  A dropped element is +0 whatever it held, and so is the gradient that reaches its place
+(x's own gradient there, unless a norm stands between: its gradient joins the whole row).
 
 Types: float32, bfloat16, float16; weight and bias in x's type or float32.  Sums, statistics and activations are float32,
 rounded once at the end.  Rows are the last dimension; rows that are evenly spaced with adjacent features are read in place,

@@ -401,8 +401,9 @@ int amber_mpn_estimate_num_elements(const int64_t* simplices, int32_t verts_per_
  * Philox-4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers, as easy as 1, 2, 3; SC 2011) under key = state[0] at
  * counter words (lo, hi of i >> 2; lo, hi of state[1] + sequence).  It is dropped iff the word is < floor(p * 2^32) (every
  * element for p = 1); a kept one is multiplied by float(1 / (1 - p)); a dropped one is +0 whatever it held (inf and NaN
- * included), and so is its gradient.  The backward pass regenerates the same words.  `state` is a DEVICE int64[2] (seed,
- * offset), so that a captured graph draws anew at every replay.
+ * included).  The gradient that reaches a dropped place is +0 as well, whatever came in: without `normalize` that is x's own
+ * gradient there, whatever act'(x) is (with it x's gradient is the norm's, which joins the whole row).  The backward pass
+ * regenerates the same words.  `state` is a DEVICE int64[2] (seed, offset), so that a captured graph draws anew at every replay.
  *
  * amber_mpn_generator_take: taken = (state[0], state[1]) and state[1] += count, one atomic step (calls on several streams
  * get disjoint ranges, in no fixed order).
