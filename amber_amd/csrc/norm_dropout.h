@@ -394,17 +394,52 @@ DEVINL void join_waves(float (&v)[N], float (&box)[W][N]) {
   }
 }
 // 1 / sqrt(v): the hardware's estimate (1 unit in the last place) and one Newton step.  The estimate takes no subnormal numbers,
-// the step no infinity: a variance below 2^-96 is scaled, an overflown one gives 0.
-DEVINL float rsqrt_of(float v) {
-  const bool tiny = v < 0x1p-96f;
-  const float u = tiny ? v * 0x1p96f : v, r = __builtin_amdgcn_rsqf(u);
-  const float q = r * fmaf(-0.5f * u * r, r, 1.5f);
-  return u > 3.0e38f ? r : tiny ? q * 0x1p48f : q;
+// the step no infinity: a variance below 2^-96 is scaled (only where eps leaves one: uniform), an overflown one gives 0.
+DEVINL float rsqrt_normal(float v) {
+  const float r = __builtin_amdgcn_rsqf(v);
+  return v > 3.0e38f ? r : r * fmaf(-0.5f * v * r, r, 1.5f);
 }
-// sum / D with inv = 1 / D rounded: one correction, so that a row of equal values has exactly that value as its mean
+DEVINL float rsqrt_of(float v, float least) {
+  if (least >= 0x1p-96f) return rsqrt_normal(v);
+  return v < 0x1p-96f ? rsqrt_normal(v * 0x1p96f) * 0x1p48f : rsqrt_normal(v);
+}
+// sum / D with inv = 1 / D rounded: one correction, so that the quotient is good to half a step
 DEVINL float mean_of(float sum, float width, float inv) {
   const float m = sum * inv;
   return fmaf(fmaf(-m, width, sum), inv, m);
+}
+// What the differences d = a - m from a first mean m add up to: m carries the rounding errors of its sum (some 2^-24 |m|, which next to
+// a small deviation is much: rows of 1000.1 with eps = 1e-5 came out at 0.04 instead of 0 for 1021 features), and the mean of d takes
+// them off again.  The variance is that of a: mean(d^2) - mean(d)^2, where the second term is as small as m's error.
+struct Spread {
+  float shift, rstd;  // mean(d): n = (d - shift) rstd, the row's mean is m + shift
+};
+DEVINL Spread spread_of(float sum, float squares, float inv, float eps) {
+  const float shift = sum * inv;
+  const float left = squares - fminf(shift * sum, 3.0e38f);  // not a difference of two infinities
+  return {shift, rsqrt_of(fmaf(fmaxf(left, 0.f), inv, eps), eps)};  // left = NaN: m is, and so is every n
+}
+// A sum of many terms one after the other, with the rounding errors of its additions beside it (Knuth's two-sum): good to some 2^-24 of
+// the terms' magnitude however many there are.  For rows whose lanes add more than a handful of packs.
+struct LongSum {
+  float s = 0.f, e = 0.f;
+  DEVINL void add(float v) {
+    const float t = s + v, z = t - s;
+    e += (s - (t - z)) + (v - z);
+    s = t;
+  }
+  DEVINL float value() const { return s - s == 0.f ? s + e : s; }  // infinite or NaN: e is NaN
+};
+template <int V>
+DEVINL float pack_sum(const float (&v)[V]) {
+  float s[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) s[j] = v[j];
+#pragma unroll
+  for (int n = V / 2; n >= 1; n /= 2)
+#pragma unroll
+    for (int j = 0; j < n; ++j) s[j] += s[j + n];
+  return s[0];
 }
 
 // Rows that no team holds in registers (beyond 16384 features): a block of 16 waves reads a row three times forward and twice
@@ -413,7 +448,7 @@ constexpr int kWide = 1024;
 template <class T>
 __global__ __launch_bounds__(kWide) void norm_forward_kernel(TailArgs a) {
   constexpr int V = kVec<T>;
-  __shared__ float box[2][kWide / 64][1];
+  __shared__ float box[kWide / 64][1], boxes[kWide / 64][2];
   Stream s{};
   if (a.drop) s = stream_of(a.state, a.sequence);
   const int width = static_cast<int>(a.width), fp32 = a.weight_dtype == AMBER_DTYPE_F32;
@@ -421,43 +456,48 @@ __global__ __launch_bounds__(kWide) void norm_forward_kernel(TailArgs a) {
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     T* y = static_cast<T*>(a.y) + row * a.width;
-    float sum[1] = {0.f}, v[V];
+    float sum[1], both[2], v[V];
     const auto load = [&](int c) {
       load_pack<false>(x + c, width - c, v);
       act_any<false>(a.act, v, v);  // 0 where the row has ended: act(0) = 0
     };
+    LongSum first;
     for (int c = threadIdx.x * V; c < width; c += kWide * V) {
       load(c);
-#pragma unroll
-      for (int j = 0; j < V; ++j) sum[0] += v[j];
+      first.add(pack_sum(v));
     }
-    sum[0] = team_sum<64>(sum[0]);
-    join_waves<kWide / 64, 1>(sum, box[0]);
+    sum[0] = team_sum<64>(first.value());
+    join_waves<kWide / 64, 1>(sum, box);
     const float mean = mean_of(sum[0], static_cast<float>(width), inv);
-    sum[0] = 0.f;
+    LongSum rest, squares;
     for (int c = threadIdx.x * V; c < width; c += kWide * V) {
       load(c);
+      float q[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = c + j < width ? v[j] - mean : 0.f;
-        sum[0] = fmaf(d, d, sum[0]);
+        v[j] = c + j < width ? v[j] - mean : 0.f;
+        q[j] = v[j] * v[j];
       }
+      rest.add(pack_sum(v));
+      squares.add(pack_sum(q));
     }
-    sum[0] = team_sum<64>(sum[0]);
-    join_waves<kWide / 64, 1>(sum, box[1]);
-    const float rstd = rsqrt_of(fmaf(sum[0], inv, a.eps));
+    both[0] = team_sum<64>(rest.value());
+    both[1] = team_sum<64>(squares.value());
+    join_waves<kWide / 64, 2>(both, boxes);
+    const Spread sp = spread_of(both[0], both[1], inv, a.eps);
     for (int c = threadIdx.x * V; c < width; c += kWide * V) {
       load(c);
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (c + j < width)
-          v[j] = fmaf((v[j] - mean) * rstd, load_weight<T>(a.weight, fp32, c + j, 1.f), load_weight<T>(a.bias, fp32, c + j, 0.f));
+          v[j] = fmaf((v[j] - mean - sp.shift) * sp.rstd, load_weight<T>(a.weight, fp32, c + j, 1.f),
+                      load_weight<T>(a.bias, fp32, c + j, 0.f));
       if (a.drop) drop_pack(a, s, row * a.width + c, v);
       store_pack<false>(y + c, width - c, v);
     }
     if (a.stats && threadIdx.x == 0) {
-      a.stats[2 * row] = mean;
-      a.stats[2 * row + 1] = rstd;
+      a.stats[2 * row] = mean + sp.shift;
+      a.stats[2 * row + 1] = sp.rstd;
     }
   }
 }
@@ -476,7 +516,8 @@ __global__ __launch_bounds__(kWide) void norm_backward_kernel(TailArgs a) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* g = static_cast<const T*>(a.g) + row * a.ldg;
     const float mean = a.stats[2 * row], rstd = a.stats[2 * row + 1];
-    float sums[2] = {0.f, 0.f}, n[V], h[V], d[V];
+    float sums[2], n[V], h[V], d[V];
+    LongSum hs, hns;
     const auto load = [&](int c) {
       load_pack<false>(x + c, width - c, n);
       load_pack<false>(g + c, width - c, h);
@@ -489,7 +530,10 @@ __global__ __launch_bounds__(kWide) void norm_backward_kernel(TailArgs a) {
       load(c);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (c + j >= width) continue;
+        if (c + j >= width) {
+          h[j] = n[j] = 0.f;
+          continue;
+        }
         if (pw) {  // a thread's own columns: nobody else touches them
           float* const at = pw + c + j;
           const bool first = row == blockIdx.x;
@@ -497,12 +541,13 @@ __global__ __launch_bounds__(kWide) void norm_backward_kernel(TailArgs a) {
           at[width] = first ? h[j] : at[width] + h[j];
         }
         h[j] *= load_weight<T>(a.weight, fp32, c + j, 1.f);
-        sums[0] += h[j];
-        sums[1] = fmaf(h[j], n[j], sums[1]);
+        n[j] *= h[j];
       }
+      hs.add(pack_sum(h));
+      hns.add(pack_sum(n));
     }
-    sums[0] = team_sum<64>(sums[0]);
-    sums[1] = team_sum<64>(sums[1]);
+    sums[0] = team_sum<64>(hs.value());
+    sums[1] = team_sum<64>(hns.value());
     join_waves<kWide / 64, 2>(sums, box[turn]);
     if (!a.y) continue;
     T* y = static_cast<T*>(a.y) + row * a.width;
@@ -583,7 +628,7 @@ struct Columns {
 template <class T, int G, int W, int K, bool SMOOTH, int CACHE>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_forward(TailArgs a) {
   constexpr int V = kVec<T>, LANES = G * W, THREADS = W == 1 ? 256 : 64 * W, TEAMS = THREADS / LANES;
-  __shared__ float box[2][W][1];
+  __shared__ float box[W][1], boxes[W][2];
   const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
   const Columns<T, LANES, K, LANES == 1, CACHE> cols(lane, static_cast<int>(a.width));
   const bool ragged = cols.ragged(), last = W == 1 || __any(cols.stores(K - 1));  // a wave without columns in the last pack skips it
@@ -619,9 +664,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_forward(TailA
       }
     }
     sum[0] = team_sum<G>(sum[0]);
-    join_waves<W, 1>(sum, box[0]);
+    join_waves<W, 1>(sum, box);
     const float mean = mean_of(sum[0], width, inv);
-    sum[0] = 0.f;
+    float both[2] = {0.f, 0.f};  // of the differences, of their squares
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (k == K - 1 && !last) break;
@@ -629,30 +674,36 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_forward(TailA
       for (int j = 0; j < V; ++j) v[k][j] -= mean;
       if (k < K - 1 || !ragged) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum[0] = fmaf(v[k][j], v[k][j], sum[0]);
+        for (int j = 0; j < V; ++j) {
+          both[0] += v[k][j];
+          both[1] = fmaf(v[k][j], v[k][j], both[1]);
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float c = cols.counts(k, j) ? v[k][j] : 0.f;
-          sum[0] = fmaf(c, c, sum[0]);
+          both[0] += c;
+          both[1] = fmaf(c, c, both[1]);
         }
       }
     }
-    sum[0] = team_sum<G>(sum[0]);
-    join_waves<W, 1>(sum, box[1]);
-    const float rstd = rsqrt_of(fmaf(sum[0], inv, a.eps));
+    both[0] = team_sum<G>(both[0]);
+    both[1] = team_sum<G>(both[1]);
+    join_waves<W, 2>(both, boxes);
+    const Spread sp = spread_of(both[0], both[1], inv, a.eps);
+    const float back = -sp.shift * sp.rstd;
     T* y = static_cast<T*>(a.y) + row * cols.width;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (k == K - 1 && !last) break;
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[k][j] = fmaf(v[k][j] * rstd, w[k][j], b[k][j]);
+      for (int j = 0; j < V; ++j) v[k][j] = fmaf(fmaf(v[k][j], sp.rstd, back), w[k][j], b[k][j]);
       if (a.drop) drop_pack(a, s, row * cols.width + cols.at[k], v[k]);
       cols.store(y, k, v[k]);
     }
     if (a.stats && lane == 0) {
-      a.stats[2 * row] = mean;
-      a.stats[2 * row + 1] = rstd;
+      a.stats[2 * row] = mean + sp.shift;
+      a.stats[2 * row + 1] = sp.rstd;
     }
   }
 }

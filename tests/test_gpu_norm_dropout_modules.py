@@ -63,3 +63,41 @@ def test_gradients_of_dropped_places_are_plus_zero(gpu_device, act, dtype):
         assert not bool(g[~keep].any()) and not bool(torch.signbit(g[~keep]).any())  # NaN counts as true
         if grad == 1.0:
             assert bool(torch.isfinite(g[keep & (x.abs() <= 4.0)]).all())
+
+
+@pytest.mark.parametrize("width", [333, 1021, 1024, 4099, 8190, 16383, 40003, 999983])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_constant_rows_whose_sum_is_not_exact(gpu_device, width, dtype):
+    """Rows of one value c: y is the bias and dx is 0 (up to the spread that the gradient alone has).  A first mean is off by some
+    k u |c|, k <= 48 (a lane's elements or a compensated sum, then a tree); what the differences from it add up to takes that off again,
+    to k u of it.  So |n| <= (48 u)^2 |c| / sqrt(eps), the statistics' mean is c to half a step, and n in the backward pass is at most
+    u |c| / sqrt(eps)."""
+    t, eps = DTYPES[dtype], 1e-5
+    rows = 3
+    gen = torch.Generator().manual_seed(width)
+    w, b = 1 + 0.2 * torch.randn(width, generator=gen), 0.2 * torch.randn(width, generator=gen)
+    go = torch.randn(rows, width, generator=gen).to(t)
+    c = torch.tensor([[1000.1], [-0.3], [7.7]]).to(t)
+    x = c.expand(rows, width).contiguous()
+    got = _run(x.to(gpu_device), None, w.to(gpu_device), b.to(gpu_device), True, 0.0, None, go.to(gpu_device))
+    cd, e = c.double().abs(), _half(t)[0]
+    n = (48 * U) ** 2 * cd / math.sqrt(eps)
+    y = got[0].cpu().double()
+    assert bool(((y - b.double()).abs() <= 1.01 * (n * w.double().abs() + (2 * U + e) * b.double().abs())).all())
+    # dx = rstd (h - mean h - n mean(h n)) with |n| <= u |c| / sqrt(eps)
+    h = go.double() * w.double()
+    r, nb = 1 / math.sqrt(eps), U * cd / math.sqrt(eps)
+    want = r * (h - h.mean(1, keepdim=True))
+    bound = r * (60 * U * (h.abs() + h.abs().mean(1, keepdim=True)) + nb * nb * h.abs().mean(1, keepdim=True)) + e * want.abs() + _half(t)[1]
+    assert bool(((got[1].cpu().double() - want).abs() <= 1.01 * bound).all())
+
+
+@pytest.mark.parametrize("rows, width", [(2, 16385), (3, 40003), (2, 999983), (1, 4194309)])
+@pytest.mark.parametrize("offset", [0.0, 300.0])
+def test_wide_rows_are_summed_as_accurately_as_narrow_ones(gpu_device, rows, width, offset):
+    """The depth of a row held in registers whatever the width: forward with a mean far from 0, backward."""
+    x, w, b, go = _data(rows, width, torch.float32, torch.float32, seed=width)
+    x, go = x + offset, go + (0.5 if offset else 0.0)
+    d = [t.to(gpu_device) for t in (x, w, b, go)]
+    got = _run(d[0], None, d[1], d[2], True, 0.0, None, d[3])
+    _compare(got, orc.tail(x, None, w, b, grad=go), _norm_bounds(x, w, b, go, chain=8))
