@@ -85,17 +85,27 @@ DEVINL void store_weight(void* w, int fp32, int64_t i, float v) {
 
 // ---------------------------------------------------------------------------------------------------
 // activations and their derivatives from the pre-activation x (torch's definitions and default arguments; at the kink of
-// relu / leakyrelu / elu the derivative from the left).  fp32 on the hardware's 2^x and reciprocal (1 unit in the last place):
-//   exp(x) = 2^(x log2 e): relative error (1.5 |x| + 1) 2^-24, which in every use below multiplies a value that falls like exp(-|x|)
+// relu / leakyrelu / elu the derivative from the left), on the hardware's 2^x and reciprocal (1 unit in the last place, 2^-23):
+//   exp(x) = 2^t (1 + d), t = x log2 e rounded, d = x - t ln 2 what the rounding left: relative error (4 + |x| / 20) 2^-24, so that
+//         silu, mish, gelu and elu's derivative keep their relative accuracy where they fall like exp(-|x|) (without d 58 2^-24 at
+//         -60).  In 16 bits (T) without it: 1.5 |x| 2^-24 more, far below the output's own 2^-12
 //   tanh: x P(x^2) below 1/2 (relative error 1.3e-8), 1 - 2 / (1 + e^2|x|) above
 //   expm1: x P(x) above -1/2 (1.4e-9), exp(x) - 1 below
 //   mish: tanh(log(1 + w)) = n / (n + 2) with w = e^x, n = w (w + 2): no cancellation; beyond x = 20 it is 1 in fp32
-//   gelu: Phi(-a) = e^(-a^2/2) t Q(t), t = 1 / (1 + 0.3 a), a = |x| (relative error 5e-8 up to a = 9): the tail itself is
-//         approximated, so x Phi(x) keeps its relative accuracy for negative x, and the derivative shares the exponential
+//   gelu: Phi(-a) = e^(-a^2/2) t Q(t), t = 1 / (1 + 0.3 a), a = |x| (Q's fit: 5e-8 up to a = 9; all of it within 20 2^-24): the tail
+//         itself is approximated, so x Phi(x) keeps its relative accuracy for negative x, and the derivative shares the exponential
 // The polynomials are least-maximum fits of these functions.
 // ---------------------------------------------------------------------------------------------------
-DEVINL float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
+template <class T>
+DEVINL float exp_of(float x) {
+  const float t = x * kLog2e, e = __builtin_amdgcn_exp2f(t);
+  if (sizeof(T) < 4) return e;
+  // |d| < 2^-15 wherever e is neither 0 nor infinite; beyond that it may be anything (inf - inf) and is held there
+  return e * (1.f + __builtin_amdgcn_fmed3f(fmaf(t, -kLn2, x), -0x1p-15f, 0x1p-15f));
+}
 DEVINL float rcp_of(float x) { return __builtin_amdgcn_rcpf(x); }
+template <class T>
 DEVINL float tanh_of(float x) {
   const float a = fabsf(x), z = x * x;
   float p = 0.01715129399739507f;
@@ -103,9 +113,10 @@ DEVINL float tanh_of(float x) {
   p = fmaf(p, z, 0.13324906927244848f);
   p = fmaf(p, z, -0.3333307579068465f);
   p = fmaf(p, z, 0.99999998737373f);
-  const float far = fmaf(-2.f, rcp_of(1.f + exp_of(2.f * a)), 1.f);
+  const float far = fmaf(-2.f, rcp_of(1.f + exp_of<T>(2.f * a)), 1.f);
   return a < 0.5f ? x * p : copysignf(far, x);
 }
+template <class T>
 DEVINL float expm1_of(float x) {  // x <= 0
   float p = 0.0011216346774701612f;
   p = fmaf(p, x, 0.008187385691190183f);
@@ -113,11 +124,12 @@ DEVINL float expm1_of(float x) {  // x <= 0
   p = fmaf(p, x, 0.16666224080228778f);
   p = fmaf(p, x, 0.4999998074594835f);
   p = fmaf(p, x, 0.9999999986263833f);
-  return x > -0.5f ? x * p : exp_of(x) - 1.f;
+  return x > -0.5f ? x * p : exp_of<T>(x) - 1.f;
 }
 struct Gelu {
   float tail, density;  // Phi(-|x|), e^(-x^2 / 2)
 };
+template <class T>
 DEVINL Gelu gelu_parts(float a) {
   const float t = rcp_of(fmaf(0.3f, a, 1.f));
   float q = 0.03753587207292055f;
@@ -128,23 +140,29 @@ DEVINL Gelu gelu_parts(float a) {
   q = fmaf(q, t, 0.09778364147982758f);
   q = fmaf(q, t, 0.12110575544066968f);
   q = fmaf(q, t, 0.1196054879202132f);
-  const float e = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f);
+  if (sizeof(T) < 4) {
+    const float e = __builtin_amdgcn_exp2f(a * a * (-0.5f * kLog2e));
+    return {t * q * e, e};
+  }
+  const float c = fminf(a, 16.f), n = -0.5f * c, h = n * c, u = h * kLog2e;  // h = -c^2 / 2; beyond 16 e is 0 (and NaN comes from t)
+  const float d = fmaf(u, -kLn2, h) + fmaf(n, c, -h), g = __builtin_amdgcn_exp2f(u), e = fmaf(g, d, g);
   return {t * q * e, e};
 }
+template <class T>
 DEVINL float act_of(float x, int act) {
   switch (act) {
     case AMBER_ACT_RELU: return x < 0.f ? 0.f : x;  // NaN stays NaN
     case AMBER_ACT_LEAKYRELU: return x > 0.f ? x : 0.01f * x;
-    case AMBER_ACT_TANH: return tanh_of(x);
-    case AMBER_ACT_ELU: return x > 0.f ? x : expm1_of(x);
-    case AMBER_ACT_SILU: return x * rcp_of(1.f + exp_of(-x));
+    case AMBER_ACT_TANH: return tanh_of<T>(x);
+    case AMBER_ACT_ELU: return x > 0.f ? x : expm1_of<T>(x);
+    case AMBER_ACT_SILU: return x * rcp_of(1.f + exp_of<T>(-x));
     case AMBER_ACT_MISH: {
-      const float w = exp_of(x > 20.f ? 20.f : x), n = w * (w + 2.f);
+      const float w = exp_of<T>(x > 20.f ? 20.f : x), n = w * (w + 2.f);
       return x * (n * rcp_of(n + 2.f));
     }
     case AMBER_ACT_GELU: {
       const float a = fabsf(x);
-      return fmaf(-fminf(a, 16.f), gelu_parts(a).tail, fmaxf(x, 0.f));
+      return fmaf(-fminf(a, 16.f), gelu_parts<T>(a).tail, fmaxf(x, 0.f));
     }
     default: return x;
   }
@@ -152,26 +170,27 @@ DEVINL float act_of(float x, int act) {
 struct ActGrad {
   float a, d;  // act(x), act'(x)
 };
+template <class T>
 DEVINL ActGrad act_grad(float x, int act) {
   switch (act) {
     case AMBER_ACT_RELU: return {x < 0.f ? 0.f : x, x > 0.f ? 1.f : 0.f};
     case AMBER_ACT_LEAKYRELU: return x > 0.f ? ActGrad{x, 1.f} : ActGrad{0.01f * x, 0.01f};
     case AMBER_ACT_TANH: {
-      const float t = tanh_of(x);
+      const float t = tanh_of<T>(x);
       return {t, fmaf(-t, t, 1.f)};
     }
-    case AMBER_ACT_ELU: return x > 0.f ? ActGrad{x, 1.f} : ActGrad{expm1_of(x), exp_of(x)};
+    case AMBER_ACT_ELU: return x > 0.f ? ActGrad{x, 1.f} : ActGrad{expm1_of<T>(x), exp_of<T>(x)};
     case AMBER_ACT_SILU: {
-      const float s = rcp_of(1.f + exp_of(-x));
+      const float s = rcp_of(1.f + exp_of<T>(-x));
       return {x * s, s * fmaf(x, 1.f - s, 1.f)};
     }
     case AMBER_ACT_MISH: {
-      const float c = x > 20.f ? 20.f : x, w = exp_of(c), n = w * (w + 2.f), r = rcp_of(n + 2.f), t = n * r;
+      const float c = x > 20.f ? 20.f : x, w = exp_of<T>(c), n = w * (w + 2.f), r = rcp_of(n + 2.f), t = n * r;
       return {x * t, fmaf(c * r, 4.f * w * (w + 1.f) * r, t)};
     }
     case AMBER_ACT_GELU: {
       const float a = fabsf(x), ac = fminf(a, 16.f);
-      const Gelu g = gelu_parts(a);
+      const Gelu g = gelu_parts<T>(a);
       return {fmaf(-ac, g.tail, fmaxf(x, 0.f)), fmaf(copysignf(ac, x), 0.39894228040143268f * g.density, x < 0.f ? g.tail : 1.f - g.tail)};
     }
     default: return {x, 1.f};
@@ -250,42 +269,42 @@ DEVINL void drop_pack(const TailArgs& a, const Stream& s, int64_t first, float (
 
 // v = act(v), d = act'(v) (if wanted) on N values: the choice is uniform and made outside the loops.  SMOOTH: the activations beyond
 // none / relu / leakyrelu, in kernels of their own (they need more registers).
-template <int ACT, bool GRAD, int N>
+template <class T, int ACT, bool GRAD, int N>
 DEVINL void act_loop(float (&v)[N], float (&d)[N]) {
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     if (GRAD) {
-      const ActGrad t = act_grad(v[j], ACT);
+      const ActGrad t = act_grad<T>(v[j], ACT);
       v[j] = t.a;
       d[j] = t.d;
     } else {
-      v[j] = act_of(v[j], ACT);
+      v[j] = act_of<T>(v[j], ACT);
     }
   }
 }
-template <bool SMOOTH, bool GRAD, int N>
+template <class T, bool SMOOTH, bool GRAD, int N>
 DEVINL void act_pack(int act, float (&v)[N], float (&d)[N]) {
   if (SMOOTH) {
     switch (act) {
-      case AMBER_ACT_TANH: return act_loop<AMBER_ACT_TANH, GRAD>(v, d);
-      case AMBER_ACT_ELU: return act_loop<AMBER_ACT_ELU, GRAD>(v, d);
-      case AMBER_ACT_SILU: return act_loop<AMBER_ACT_SILU, GRAD>(v, d);
-      case AMBER_ACT_MISH: return act_loop<AMBER_ACT_MISH, GRAD>(v, d);
-      default: return act_loop<AMBER_ACT_GELU, GRAD>(v, d);
+      case AMBER_ACT_TANH: return act_loop<T, AMBER_ACT_TANH, GRAD>(v, d);
+      case AMBER_ACT_ELU: return act_loop<T, AMBER_ACT_ELU, GRAD>(v, d);
+      case AMBER_ACT_SILU: return act_loop<T, AMBER_ACT_SILU, GRAD>(v, d);
+      case AMBER_ACT_MISH: return act_loop<T, AMBER_ACT_MISH, GRAD>(v, d);
+      default: return act_loop<T, AMBER_ACT_GELU, GRAD>(v, d);
     }
   }
   switch (act) {
-    case AMBER_ACT_RELU: return act_loop<AMBER_ACT_RELU, GRAD>(v, d);
-    case AMBER_ACT_LEAKYRELU: return act_loop<AMBER_ACT_LEAKYRELU, GRAD>(v, d);
-    default: return act_loop<AMBER_ACT_NONE, GRAD>(v, d);
+    case AMBER_ACT_RELU: return act_loop<T, AMBER_ACT_RELU, GRAD>(v, d);
+    case AMBER_ACT_LEAKYRELU: return act_loop<T, AMBER_ACT_LEAKYRELU, GRAD>(v, d);
+    default: return act_loop<T, AMBER_ACT_NONE, GRAD>(v, d);
   }
 }
 
 inline __host__ __device__ bool is_smooth(int act) { return act != AMBER_ACT_NONE && act != AMBER_ACT_RELU && act != AMBER_ACT_LEAKYRELU; }
-template <bool GRAD, int N>
+template <class T, bool GRAD, int N>
 DEVINL void act_any(int act, float (&v)[N], float (&d)[N]) {
-  if (is_smooth(act)) act_pack<true, GRAD>(act, v, d);
-  else act_pack<false, GRAD>(act, v, d);
+  if (is_smooth(act)) act_pack<T, true, GRAD>(act, v, d);
+  else act_pack<T, false, GRAD>(act, v, d);
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -312,10 +331,10 @@ __global__ __launch_bounds__(kBlock) void elementwise_kernel(TailArgs a) {
   if (a.drop) s = stream_of(a.state, a.sequence);
   // v = what the dropout applies to, z = the pre-activation
   const auto work = [&](float (&v)[V], float (&z)[V], int64_t first) {
-    if (!BWD) act_pack<SMOOTH, false>(a.act, v, v);
+    if (!BWD) act_pack<T, SMOOTH, false>(a.act, v, v);
     if (BWD && a.act != AMBER_ACT_NONE) {
       float d[V];
-      act_pack<SMOOTH, true>(a.act, z, d);
+      act_pack<T, SMOOTH, true>(a.act, z, d);
       if (a.drop) {  // selected last: the derivative may be negative (-0), NaN or infinite where the gradient is 0
         select_pack(a, s, first, v, [&](int j) { return v[j] * a.scale * d[j]; });
       } else {
@@ -459,7 +478,7 @@ __global__ __launch_bounds__(kWide) void norm_forward_kernel(TailArgs a) {
     float sum[1], both[2], v[V];
     const auto load = [&](int c) {
       load_pack<false>(x + c, width - c, v);
-      act_any<false>(a.act, v, v);  // 0 where the row has ended: act(0) = 0
+      act_any<T, false>(a.act, v, v);  // 0 where the row has ended: act(0) = 0
     };
     LongSum first;
     for (int c = threadIdx.x * V; c < width; c += kWide * V) {
@@ -521,7 +540,7 @@ __global__ __launch_bounds__(kWide) void norm_backward_kernel(TailArgs a) {
     const auto load = [&](int c) {
       load_pack<false>(x + c, width - c, n);
       load_pack<false>(g + c, width - c, h);
-      act_any<true>(a.act, n, d);
+      act_any<T, true>(a.act, n, d);
       if (a.drop) drop_pack(a, s, row * a.width + c, h);
 #pragma unroll
       for (int j = 0; j < V; ++j) n[j] = (n[j] - mean) * rstd;
@@ -654,7 +673,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_forward(TailA
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (k == K - 1 && !last) break;
-      act_pack<SMOOTH, false>(a.act, v[k], v[k]);
+      act_pack<T, SMOOTH, false>(a.act, v[k], v[k]);
       if (k < K - 1 || !ragged) {
 #pragma unroll
         for (int j = 0; j < V; ++j) sum[0] += v[k][j];
@@ -765,7 +784,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void norm_rows_backward(Tail
     for (int k = 0; k < K; ++k) {
       if (k == K - 1 && !last) break;
       if (a.drop) drop_pack(a, s, row * cols.width + cols.at[k], h[k]);
-      act_pack<SMOOTH, true>(a.act, n[k], dact[k]);
+      act_pack<T, SMOOTH, true>(a.act, n[k], dact[k]);
 #pragma unroll
       for (int j = 0; j < V; ++j) n[k][j] = (n[k][j] - mean) * rstd;
       if (IN_LDS) {

@@ -101,3 +101,27 @@ def test_wide_rows_are_summed_as_accurately_as_narrow_ones(gpu_device, rows, wid
     d = [t.to(gpu_device) for t in (x, w, b, go)]
     got = _run(d[0], None, d[1], d[2], True, 0.0, None, d[3])
     _compare(got, orc.tail(x, None, w, b, grad=go), _norm_bounds(x, w, b, go, chain=8))
+
+
+@pytest.mark.parametrize("act, low, steps", [("silu", -60.0, 8), ("mish", -60.0, 13), ("gelu", -9.0, 18)])
+def test_negative_tails_keep_their_relative_accuracy(gpu_device, act, low, steps):
+    """fp32, relative to the value itself, which falls like exp(-|x|).  In u = 2^-24, the hardware's 2^x and reciprocal being within one
+    unit in the last place (2 u): exp 4 (2^x, 1 + d, their product) and ln 2's own rounding, 1.9e-9 log2 e |x| = |x| / 20.  silu: 4 + 1
+    (1 + e) + 2 (reciprocal) + 1.  mish: 4 x 4/3 (n = w (w + 2)) + 2 + 1 + 2 + 2, and 4/3 of ln 2's.  gelu: density 4, t 3 x 2.5 (how
+    strongly t Q(t) depends on t), Horner's scheme 2.7, the fit 0.9, three products 3, ln 2's for x^2 / 2."""
+    x = torch.linspace(low, -0.5, 200003)
+    want = orc.act(x.double(), act)
+    if act == "gelu":  # x Phi(x) by the complementary error function: 1 + erf(x) cancels
+        want = 0.5 * x.double() * torch.erfc(-x.double() / math.sqrt(2.0))
+    got = nd.activate_norm_dropout(x.to(gpu_device), act, normalize=False).cpu().double()
+    power = x.double() ** 2 / 2 if act == "gelu" else x.double().abs() * (4 / 3 if act == "mish" else 1)
+    worst = float((((got - want) / want).abs() / (U * (steps + power / 20))).max())
+    assert worst <= 1.01, worst
+
+
+def test_elu_derivative_keeps_its_relative_accuracy(gpu_device):
+    """exp(x) within (4 + |x| / 20) u of itself (above)."""
+    x = torch.linspace(-60.0, -1e-3, 200003)
+    xd = x.to(gpu_device).requires_grad_()
+    g, = torch.autograd.grad(nd.activate_norm_dropout(xd, "elu", normalize=False), xd, torch.ones_like(xd))
+    assert float(((g.cpu().double() / x.double().exp() - 1).abs() / (4 + x.double().abs() / 20)).max()) <= 1.01 * U
