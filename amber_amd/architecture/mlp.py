@@ -10,7 +10,7 @@ from torch import nn as nn
 from torch.nn.utils import spectral_norm as apply_spectral_norm
 from torch.nn.utils.spectral_norm import SpectralNorm
 
-from amber_amd.norm_dropout import CounterGenerator, activate_norm_dropout, dropout
+from amber_amd.norm_dropout import CounterGenerator, activate_norm_dropout
 
 _ACTIVATIONS = {"relu": nn.ReLU, "leakyrelu": nn.LeakyReLU, "elu": nn.ELU, "swish": nn.SiLU, "silu": nn.SiLU,
                 "mish": nn.Mish, "gelu": nn.GELU, "tanh": nn.Tanh}
@@ -47,6 +47,24 @@ def build_mlp(*, in_features: int, mlp_config, latent_dimension: int) -> nn.Modu
             layers.append(nn.Dropout(p=dropout))
         fan_in = latent_dimension
     return layers
+
+
+def _as_built(module: nn.Module, kind: type) -> bool:
+    """Whether calling `module` does what `kind` does and nothing else: no other forward, no hooks of its own."""
+    return (isinstance(module, kind) and type(module).forward is kind.forward and "forward" not in vars(module)
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
+
+
+# what an activation module has to hold for activate_norm_dropout to compute the same
+_FUSED = {nn.ReLU: ("relu", {}), nn.LeakyReLU: ("leakyrelu", {"negative_slope": 0.01}), nn.Tanh: ("tanh", {}),
+          nn.ELU: ("elu", {"alpha": 1.0}), nn.SiLU: ("silu", {}), nn.Mish: ("mish", {}), nn.GELU: ("gelu", {"approximate": "none"})}
+
+
+def _fused_activation(module: nn.Module) -> Optional[str]:
+    name, held = _FUSED.get(type(module), (None, None))
+    if name is None or not _as_built(module, type(module)) or any(getattr(module, k) != v for k, v in held.items()):
+        return None
+    return name
 
 
 class MLP(nn.Module):
@@ -113,32 +131,37 @@ class MLP(nn.Module):
         return pieces, sources
 
     def run_layers(self, tensor: torch.Tensor, generator: Optional[CounterGenerator] = None) -> torch.Tensor:
-        """The layers one by one, as the reference's MLP.forward (mlp.py:128-129).  With a generator everything after a
-        Linear is one pass (activation, LayerNorm, dropout from the counter-based generator); BatchNorm stays torch's."""
+        """The layers one by one, as the reference's MLP.forward (mlp.py:128-129).  With a generator what follows a Linear is one
+        pass (activation, LayerNorm, dropout from the counter-based generator) as far as the modules are what that pass computes; a
+        module with other parameters, a forward or hooks of its own, and BatchNorm, run by themselves.  (Hooks that torch registers
+        for all modules at once see only those.)"""
         if generator is None:
             for layer in self.mlp_layers:
                 tensor = layer(tensor)
             return tensor
         mods = list(self.mlp_layers)
-        drops = sum(isinstance(m, nn.Dropout) and m.training and m.p > 0 for m in mods)
-        state = generator.take(drops) if drops else None
-        sequence = 0
-        for i, lin in enumerate(mods):
-            if not isinstance(lin, nn.Linear):
+        drops = [m for m in mods if isinstance(m, nn.Dropout) and m.training and m.p > 0]
+        if not all(_as_built(m, nn.Dropout) for m in drops):
+            raise RuntimeError("amber_amd: a Dropout module with hooks or a forward of its own draws from torch's generator; remove them "
+                               "or use dropout_generator: torch")
+        state = generator.take(len(drops)) if drops else None
+        i = sequence = 0
+        while i < len(mods):
+            first, act, ln, p = i, _fused_activation(mods[i]), None, 0.0
+            i += act is not None
+            if i < len(mods) and _as_built(mods[i], nn.LayerNorm) and len(mods[i].normalized_shape) == 1:
+                ln = mods[i]
+                i += 1
+            if i < len(mods) and mods[i] in drops:
+                p = mods[i].p
+                i += 1
+            if i == first or (i == first + 1 and act is not None and i < len(mods) and isinstance(mods[i], nn.BatchNorm1d)):
+                tensor, i = mods[first](tensor), first + 1
                 continue
-            tail = mods[i + 2:next((j for j in range(i + 1, len(mods)) if isinstance(mods[j], nn.Linear)), len(mods))]
-            ln = next((m for m in tail if isinstance(m, nn.LayerNorm)), None)
-            bn = next((m for m in tail if isinstance(m, nn.BatchNorm1d)), None)
-            drop = next((m for m in tail if isinstance(m, nn.Dropout) and m.training and m.p > 0), None)
-            p = drop.p if drop is not None else 0.0
-            tensor = lin(tensor)
-            if bn is not None:
-                tensor = dropout(bn(mods[i + 1](tensor)), p, state, sequence=sequence)
-            else:
-                tensor = activate_norm_dropout(tensor, self.activation_function, ln.weight if ln is not None else None,
-                                               ln.bias if ln is not None else None, normalize=ln is not None,
-                                               eps=ln.eps if ln is not None else 0.0, p=p, state=state, sequence=sequence)
-            sequence += drop is not None
+            tensor = activate_norm_dropout(tensor, act, ln.weight if ln is not None else None, ln.bias if ln is not None else None,
+                                           normalize=ln is not None, eps=ln.eps if ln is not None else 0.0, p=p, state=state,
+                                           sequence=sequence)
+            sequence += p > 0
         return tensor
 
     def forward(self, tensor: torch.Tensor) -> torch.Tensor:

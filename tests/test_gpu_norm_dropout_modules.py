@@ -125,3 +125,72 @@ def test_elu_derivative_keeps_its_relative_accuracy(gpu_device):
     xd = x.to(gpu_device).requires_grad_()
     g, = torch.autograd.grad(nd.activate_norm_dropout(xd, "elu", normalize=False), xd, torch.ones_like(xd))
     assert float(((g.cpu().double() / x.double().exp() - 1).abs() / (4 + x.double().abs() / 20)).max()) <= 1.01 * U
+
+
+@pytest.mark.parametrize("change", ["slope", "alpha", "approximate", "swapped", "act_hook", "norm_hook", "norm_pre_hook", "act_forward",
+                                    "no_affine", "idle_dropout_hook"])
+def test_decoder_layers_follow_their_modules(gpu_device, change):
+    """run_layers with a generator computes what the modules in the list stand for at the call: parameters changed or modules exchanged
+    after construction, hooks, a forward of their own.  Against the modules one by one in float64, with the generator's masks."""
+    import copy
+    nn = torch.nn
+    act = {"slope": "leakyrelu", "alpha": "elu", "approximate": "gelu"}.get(change, "tanh")
+    torch.manual_seed(8)
+    mlp = MLP(in_features=64, latent_dimension=64, mlp_config=_decoder("layer", 0.25, act)).to(gpu_device).train()
+    seen, mods = [], mlp.mlp_layers  # Linear, activation, LayerNorm, Dropout, twice
+    if change == "slope":
+        mods[1].negative_slope = 0.4
+    elif change == "alpha":
+        mods[5].alpha = 0.5
+    elif change == "approximate":
+        mods[1].approximate = "tanh"
+    elif change == "swapped":
+        mods[5] = nn.Softplus()
+    elif change == "no_affine":
+        mods[2] = nn.LayerNorm(64, elementwise_affine=False, eps=1e-2)
+    elif change == "act_forward":
+        mods[1].forward = lambda t: t * 2
+    ref = copy.deepcopy(mlp).cpu().double()
+    for m in (mods, ref.mlp_layers):
+        if change == "act_hook":
+            m[1].register_forward_hook(lambda mod, args, out: (seen.append(1), out * 3)[1])
+        elif change == "norm_hook":
+            m[2].register_forward_hook(lambda mod, args, out: (seen.append(1), out * 3)[1])
+        elif change == "norm_pre_hook":
+            m[6].register_forward_pre_hook(lambda mod, args: (seen.append(1), args[0] * args[0])[1])
+        elif change == "idle_dropout_hook":  # not drawing: runs as the module it is
+            m[3].p = 0.0
+            m[3].register_forward_hook(lambda mod, args, out: (seen.append(1), out * 3)[1])
+    x, go = torch.randn(200, 64), torch.randn(200, 64)
+    xd = x.to(gpu_device).requires_grad_()
+    gen = nd.CounterGenerator(3, device=gpu_device)
+    y = mlp.run_layers(xd, gen)
+    assert len(seen) == ("hook" in change)
+    params = [q for q in mlp.parameters()]
+    grads = torch.autograd.grad(y, [xd] + params, go.to(gpu_device))
+    t = xr = x.double().requires_grad_()
+    k = 0
+    for layer in ref.mlp_layers:
+        if isinstance(layer, nn.Dropout) and layer.p > 0:
+            t = torch.where(orc.keep(t.numel(), 0.25, 3, k).view(t.shape), t / 0.75, torch.zeros((), dtype=torch.float64))
+            k += 1
+        else:
+            t = layer(t)
+    want = torch.autograd.grad(t, [xr] + list(ref.parameters()), go.double())
+    assert gen.get_state() == (3, k)
+    for name, a, r in zip(["y", "dx"] + [n for n, _ in mlp.named_parameters()], (y.detach(),) + grads, (t.detach(),) + want):
+        if change == "slope" and name == "dx":
+            continue  # a value within rounding of the kink takes the other slope
+        assert float((a.cpu().double() - r).abs().max()) <= 2e-5 * float(r.abs().max()) + 1e-7, name
+
+
+def test_hooks_on_a_drawing_dropout_are_refused(gpu_device):
+    """The module itself would draw from torch's generator."""
+    mlp = MLP(in_features=64, latent_dimension=64, mlp_config=_decoder("layer", 0.25, "tanh")).to(gpu_device).train()
+    gen = nd.CounterGenerator(3, device=gpu_device)
+    handle = mlp.mlp_layers[7].register_forward_hook(lambda mod, args, out: out)
+    with pytest.raises(RuntimeError, match="dropout_generator"):
+        mlp.run_layers(torch.randn(5, 64, device=gpu_device), gen)
+    assert gen.get_state() == (3, 0)  # refused before anything is drawn
+    handle.remove()
+    mlp.run_layers(torch.randn(5, 64, device=gpu_device), gen)
