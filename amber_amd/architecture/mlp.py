@@ -144,7 +144,7 @@ class MLP(nn.Module):
         if not all(_as_built(m, nn.Dropout) for m in drops):
             raise RuntimeError("amber_amd: a Dropout module with hooks or a forward of its own draws from torch's generator; remove them "
                                "or use dropout_generator: torch")
-        state = generator.take(len(drops)) if drops else None
+        state = generator.take_in_module(len(drops)) if drops else None
         i = sequence = 0
         while i < len(mods):
             first, act, ln, p = i, _fused_activation(mods[i]), None, 0.0

@@ -22,7 +22,7 @@ def dropout_edge(edge_index: torch.Tensor, p: float = 0.5, training: bool = True
     if not training or p == 0.0:
         return edge_index, edge_index.new_ones(num_edges, dtype=torch.bool)
     if generator is not None:
-        edge_mask = keep_mask(num_edges, p, generator.take())
+        edge_mask = keep_mask(num_edges, p, generator.take_in_module())
     else:
         edge_mask = torch.rand(num_edges, device=edge_index.device) >= p
     return edge_index[:, edge_mask], edge_mask

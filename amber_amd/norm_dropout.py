@@ -21,11 +21,16 @@ Inside a HIP graph: `take` and the operators may be captured; the generator's st
 new numbers.  Capturing a backward pass follows torch's own rule: no autograd graph that was recorded outside the capture may
 still hold the same leaves.
 
-Recomputing (torch.utils.checkpoint): call `take` outside the recomputed function and hand its result in; a `take` that is run
-again draws other numbers.
+Recomputing (torch.utils.checkpoint): a `take` that is run again draws other numbers.  Call it outside the recomputed function and hand
+its result in, or have the recomputation take the same ranges:
+
+    checkpoint(function, x, use_reentrant=False, context_fn=gen.checkpoint_contexts)
+
+The framework's own modules (decoder layers, edge dropout) take ranges inside their forward and refuse to do so anew in a backward pass.
 """
 from __future__ import annotations
 
+import threading
 from typing import Optional
 
 import torch
@@ -48,6 +53,52 @@ def _signed(value: int) -> int:
     return value - (1 << 64) if value >> 63 else value
 
 
+_thread = threading.local()  # .contexts: the _Recorded / _Replayed that are open on this thread, the innermost last
+
+
+def _take(generator, count: int, depth: Optional[int] = None) -> torch.Tensor:
+    """The next `count` ranges as the innermost of the first `depth` open contexts has them, or the generator itself."""
+    contexts = getattr(_thread, "contexts", ())
+    for i in range(len(contexts) if depth is None else depth, 0, -1):
+        if contexts[i - 1].generator is generator:
+            return contexts[i - 1].take(count, i - 1)
+    return _lib.binding().generator_take(generator.state, count)
+
+
+class _Recorded:
+    """While open: what is taken from the generator is kept in `taken`."""
+
+    def __init__(self, generator, taken: list):
+        self.generator, self.taken = generator, taken
+
+    def __enter__(self):
+        if not hasattr(_thread, "contexts"):
+            _thread.contexts = []
+        _thread.contexts.append(self)
+
+    def __exit__(self, *exc):
+        _thread.contexts.pop()
+
+    def take(self, count: int, depth: int) -> torch.Tensor:
+        state = _take(self.generator, count, depth)  # a checkpoint inside a recomputed one records what that one replays
+        self.taken.append((count, state))
+        return state
+
+
+class _Replayed(_Recorded):
+    """While open: the ranges of `taken` once more, in their order."""
+
+    def __enter__(self):
+        super().__enter__()
+        self.next = 0
+
+    def take(self, count: int, depth: int) -> torch.Tensor:
+        if self.next >= len(self.taken) or self.taken[self.next][0] != count:
+            raise RuntimeError("amber_amd: the recomputed pass takes other ranges than the first one")
+        self.next += 1
+        return self.taken[self.next - 1][1]
+
+
 class CounterGenerator(nn.Module):
     """(seed, offset) of the counter-based generator in a device buffer (not part of a state_dict: get_state / set_state).
     Two generators with one seed draw the same numbers: ranks that see different data should get different seeds."""
@@ -60,7 +111,22 @@ class CounterGenerator(nn.Module):
 
     def take(self, count: int = 1) -> torch.Tensor:
         """The next `count` ranges: int64[2] (seed, offset), to be used with sequence = 0 .. count - 1."""
-        return _lib.binding().generator_take(self.state, count)
+        return _take(self, count)
+
+    def take_in_module(self, count: int = 1) -> torch.Tensor:
+        """`take` for a module's forward pass.  Inside a backward pass, where only a recomputation runs it, the ranges of the first pass
+        or a RuntimeError: another mask would belong to other gradients."""
+        if torch._C._current_graph_task_id() != -1 and not any(isinstance(c, _Replayed) and c.generator is self
+                                                               for c in getattr(_thread, "contexts", ())):
+            raise RuntimeError("amber_amd: a recomputed forward pass would draw other numbers than the first one; call "
+                               "torch.utils.checkpoint.checkpoint with use_reentrant=False and context_fn=generator.checkpoint_contexts")
+        return _take(self, count)
+
+    def checkpoint_contexts(self):
+        """context_fn of torch.utils.checkpoint.checkpoint(..., use_reentrant=False): a pair of contexts, for the first pass and for its
+        recomputations, which take the ranges that the first pass took."""
+        taken: list = []
+        return _Recorded(self, taken), _Replayed(self, taken)
 
     def get_state(self):
         """(seed, offset) as Python ints (reads the device)."""

@@ -194,3 +194,72 @@ def test_hooks_on_a_drawing_dropout_are_refused(gpu_device):
     assert gen.get_state() == (3, 0)  # refused before anything is drawn
     handle.remove()
     mlp.run_layers(torch.randn(5, 64, device=gpu_device), gen)
+
+
+def _decoder_and_edges(gpu_device):
+    torch.manual_seed(6)
+    mlp = MLP(in_features=64, latent_dimension=64, mlp_config=_decoder("layer", 0.3, "silu")).to(gpu_device).train()
+    return mlp, torch.randn(300, 64, device=gpu_device), torch.arange(2000, device=gpu_device).view(2, 1000) % 300
+
+
+def test_recomputed_modules_draw_their_ranges_again(gpu_device):
+    """torch.utils.checkpoint around modules that take ranges themselves (decoder layers, edge dropout): with the generator's contexts the
+    outputs, the gradients and the generator's state are those of the plain call, nested checkpoints too; without them the recomputation is
+    refused instead of drawing another mask."""
+    from amber_amd.mpn.common.edge_dropout import dropout_edge
+    mlp, x, edges = _decoder_and_edges(gpu_device)
+    gen = nd.CounterGenerator(12, device=gpu_device)
+    check = torch.utils.checkpoint.checkpoint
+
+    def layers(t):
+        return mlp.run_layers(t, gen)
+
+    def whole(t):
+        _, kept = dropout_edge(edges, 0.4, True, gen)
+        return layers(t) * kept[:300, None]
+
+    def nested(t):
+        return check(layers, check(whole, t, use_reentrant=False, context_fn=gen.checkpoint_contexts), use_reentrant=False,
+                     context_fn=gen.checkpoint_contexts)
+
+    def gradients(f):
+        gen.set_state(12, 40)
+        xl = x.clone().requires_grad_()
+        y = f(xl)
+        state = gen.get_state()
+        return (y.detach(),) + torch.autograd.grad(y.square().sum(), [xl] + list(mlp.parameters())) + (state,)
+
+    for f in (layers, whole, lambda t: layers(whole(t)), nested):
+        plain = nested if f is nested else f
+        want = gradients((lambda t: layers(whole(t))) if f is nested else f)
+        got = gradients(nested if f is nested else lambda t: check(plain, t, use_reentrant=False, context_fn=gen.checkpoint_contexts))
+        assert all(torch.equal(a, b) for a, b in zip(want[:-1], got[:-1])) and want[-1] == got[-1] == gen.get_state()
+    both = lambda t: check(nested, t, use_reentrant=False, context_fn=gen.checkpoint_contexts)  # three deep
+    assert all(torch.equal(a, b) for a, b in zip(want[:-1], gradients(both)[:-1]))
+    for f in (layers, whole):
+        for reentrant in (False, True):
+            with pytest.raises(RuntimeError, match="checkpoint_contexts"):
+                check(f, x.clone().requires_grad_(), use_reentrant=reentrant).sum().backward()
+    gradients(layers)  # nothing is left open
+
+
+def test_recomputed_model_draws_its_ranges_again(gpu_device):
+    """The same around a whole SupervisedMPN: edge dropout and decoder dropout of one generator."""
+    g = syn.grid_batch(num_graphs=2, nx=9, ny=8, in_node_features=5, in_edge_features=2).to(gpu_device)
+    cfg = default_architecture(latent_dimension=64, num_steps=2)
+    cfg["decoder"] = _decoder("layer", 0.2, "leakyrelu")
+    torch.manual_seed(5)
+    model = SupervisedMPN(AttrDict(cfg, dropout_generator="counter", dropout_seed=7), g).to(gpu_device).train()
+    gen = model.mpn.dropout_generator
+    anchor = torch.zeros((), device=gpu_device, requires_grad=True)  # something to differentiate among the checkpoint's arguments
+
+    def step(**kw):
+        gen.set_state(7, 9)
+        f = lambda a: model(g) + a
+        out = f(anchor) if not kw else torch.utils.checkpoint.checkpoint(f, anchor, use_reentrant=False, **kw)
+        return (out.detach(),) + torch.autograd.grad(out.square().mean(), list(model.parameters()))
+
+    want, got = step(), step(context_fn=gen.checkpoint_contexts)
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and gen.get_state() == (7, 12)
+    with pytest.raises(RuntimeError, match="checkpoint_contexts"):
+        step(determinism_check="default")

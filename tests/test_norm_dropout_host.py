@@ -237,3 +237,33 @@ def test_world_size_2_broadcast_leaves_each_rank_its_generator():
     ret = mp.Manager().dict()
     mp.spawn(_broadcast_worker, args=(port, ret), nprocs=2, join=True)
     assert ret[0] == ([1.0] * 3, (40, 0)) and ret[1] == ([1.0] * 3, (41, 0))
+
+
+def test_taking_anew_inside_a_backward_pass_is_refused():
+    gen = nd.CounterGenerator(3)
+
+    class Again(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            gen.take_in_module()
+
+    with pytest.raises(RuntimeError, match="checkpoint_contexts"):
+        Again.apply(torch.ones(2, requires_grad=True)).sum().backward()
+    first, again = gen.checkpoint_contexts()
+    with again, pytest.raises(RuntimeError, match="other ranges"):  # more than the first pass took
+        gen.take()
+    with first, pytest.raises(RuntimeError, match="MI355X only"):  # the generator itself is asked
+        gen.take()
+
+
+def test_drawing_dropout_with_hooks_is_refused():
+    cfg = AttrDict({"activation_function": "tanh", "num_layers": 1,
+                    "regularization": {"dropout": 0.5, "spectral_norm": False, "latent_normalization": None}})
+    mlp = MLP(in_features=8, latent_dimension=8, mlp_config=cfg)
+    mlp.mlp_layers[2].register_forward_pre_hook(lambda mod, args: None)
+    with pytest.raises(RuntimeError, match="dropout_generator"):
+        mlp.run_layers(torch.randn(4, 8), nd.CounterGenerator(1))
