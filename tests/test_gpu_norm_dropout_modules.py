@@ -263,3 +263,34 @@ def test_recomputed_model_draws_its_ranges_again(gpu_device):
     assert all(torch.equal(a, b) for a, b in zip(want, got)) and gen.get_state() == (7, 12)
     with pytest.raises(RuntimeError, match="checkpoint_contexts"):
         step(determinism_check="default")
+
+
+def test_decoder_layers_with_leaky_relu_everywhere_but_at_the_kink(gpu_device):
+    """MLP.run_layers with the default activation: the output in all rows, the gradient in every row none of whose pre-activations lies
+    within 1e-5 of the kink (they are off by less: products of 64 terms of order 1, a few u sqrt(64)).  2e-5 of the largest value, as in
+    test_decoder_layers_in_one_pass_each."""
+    import copy
+    torch.manual_seed(4)
+    mlp = MLP(in_features=64, latent_dimension=64, mlp_config=_decoder("layer", 0.3, "leakyrelu")).to(gpu_device).train()
+    with torch.no_grad():
+        for q in mlp.parameters():
+            q.add_(0.1 * torch.randn_like(q))
+    x = torch.randn(700, 64, device=gpu_device, requires_grad=True)
+    go = torch.randn(700, 64, device=gpu_device)
+    ref = copy.deepcopy(mlp).cpu().double()
+    y = mlp.run_layers(x, nd.CounterGenerator(31, device=gpu_device))
+    dx, = torch.autograd.grad(y, x, go)
+    t = xr = x.detach().cpu().double().requires_grad_()
+    k, clear = 0, torch.ones(700, dtype=torch.bool)
+    for layer in ref.mlp_layers:
+        if isinstance(layer, torch.nn.Dropout):
+            t = torch.where(orc.keep(t.numel(), 0.3, 31, k).view(t.shape), t / 0.7, torch.zeros((), dtype=torch.float64))
+            k += 1
+            continue
+        if isinstance(layer, torch.nn.LeakyReLU):
+            clear &= (t.detach().abs() > 1e-5).all(1)
+        t = layer(t)
+    want, = torch.autograd.grad(t, xr, go.cpu().double())
+    assert int(clear.sum()) > 650
+    assert float((y.detach().cpu().double() - t.detach()).abs().max()) <= 2e-5 * float(t.detach().abs().max())
+    assert float((dx.cpu().double() - want)[clear].abs().max()) <= 2e-5 * float(want.abs().max())
