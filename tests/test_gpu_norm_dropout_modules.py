@@ -294,3 +294,15 @@ def test_decoder_layers_with_leaky_relu_everywhere_but_at_the_kink(gpu_device):
     assert int(clear.sum()) > 650
     assert float((y.detach().cpu().double() - t.detach()).abs().max()) <= 2e-5 * float(t.detach().abs().max())
     assert float((dx.cpu().double() - want)[clear].abs().max()) <= 2e-5 * float(want.abs().max())
+
+
+@pytest.mark.parametrize("rows, width", [(4, 64), (63, 64), (20736, 64), (30011, 128), (6000, 1021), (3001, 8190), (2000, 16385)])
+def test_weight_gradients_of_many_rows_lose_no_block(gpu_device, rows, width):
+    """The sums over rows within the depth that they are added with: at least 256 blocks share the rows where there are many, a block's
+    rows follow one another, then at most 64 additions join lanes, waves and blocks.  A block's sum missing or counted twice is far
+    beyond that: every row adds g in [0.5, 1.5] to dbias, and as much times n to dweight."""
+    x, w, b, go = _data(rows, width, torch.float32, torch.float32, seed=rows)
+    go = go.clamp(-1, 1) / 2 + 1
+    d = [t.to(gpu_device) for t in (x, w, b, go)]
+    got = _run(d[0], None, d[1], d[2], True, 0.0, None, d[3])
+    _compare(got, orc.tail(x, None, w, b, grad=go), _norm_bounds(x, w, b, go, chain=64 + rows // 256))
