@@ -310,7 +310,7 @@ DEVINL void act_any(int act, float (&v)[N], float (&d)[N]) {
 // ---------------------------------------------------------------------------------------------------
 // without the norm: elementwise over the flat tensor, 16 bytes a thread, the next 16 on their way while these are worked on
 // (32768 x 4096 fp32 dropout 189 -> 177 us, 6.1 TB/s; 1.44 M x 128 fp32 with an activation 264 -> 245 forward, 446 -> 370 backward).
-// Bound by the memory; relu and leaky relu cost nothing beside it, gelu in 16 bits does (1000003 x 333 fp16 with dropout 4.0 TB/s).
+// Bound by the memory; relu and leaky relu cost nothing beside it, gelu in fp32 2 % (248 us forward), in 16 bits more (1000003 x 333 fp16 with dropout 4.0 TB/s).
 // ---------------------------------------------------------------------------------------------------
 template <class T, bool BWD, bool SMOOTH, int CACHE>
 __global__ __launch_bounds__(kBlock) void elementwise_kernel(TailArgs a) {
@@ -429,7 +429,8 @@ DEVINL float mean_of(float sum, float width, float inv) {
 }
 // What the differences d = a - m from a first mean m add up to: m carries the rounding errors of its sum (some 2^-24 |m|, which next to
 // a small deviation is much: rows of 1000.1 with eps = 1e-5 came out at 0.04 instead of 0 for 1021 features), and the mean of d takes
-// them off again.  The variance is that of a: mean(d^2) - mean(d)^2, where the second term is as small as m's error.
+// them off again (1440000 x 128 fp32 forward 237 us either way, 243 -> 250 with dropout, which asks for its vector instructions; 5003 x
+// 4099 bf16 19.7 -> 20.5).  The variance is that of a: mean(d^2) - mean(d)^2, where the second term is as small as m's error.
 struct Spread {
   float shift, rstd;  // mean(d): n = (d - shift) rstd, the row's mean is m + shift
 };
@@ -439,7 +440,8 @@ DEVINL Spread spread_of(float sum, float squares, float inv, float eps) {
   return {shift, rsqrt_of(fmaf(fmaxf(left, 0.f), inv, eps), eps)};  // left = NaN: m is, and so is every n
 }
 // A sum of many terms one after the other, with the rounding errors of its additions beside it (Knuth's two-sum): good to some 2^-24 of
-// the terms' magnitude however many there are.  For rows whose lanes add more than a handful of packs.
+// the terms' magnitude however many there are.  For rows whose lanes add more than a handful of packs (20 x 999983 fp32 forward 708 us
+// before, 693 with it and a pack's terms added pairwise).
 struct LongSum {
   float s = 0.f, e = 0.f;
   DEVINL void add(float v) {
@@ -911,10 +913,10 @@ inline Shape shape_for(int64_t width, int vec) {
 inline int64_t teams_in_block(const Shape& h) { return h.w > 1 ? 1 : 256 / h.g; }
 // Blocks of a launch: each takes rows in turn and has the next ones on their way, so their number sets the bytes in flight.  About
 // 4 MB forward and 6 MB backward (x and the gradient) are best; more only spread the accesses over more pages: 1.44 M x 128 fp32
-// forward 250 us with 1024 blocks, 311 with 512, 328 with 2048 (before its accesses went past the caches: 244 us now, 6.0 TB/s);
+// forward 250 us with 1024 blocks, 311 with 512, 328 with 2048 (before its accesses went past the caches: 237 us now, 6.2 TB/s);
 // 100000 x 1024 fp32 backward 219 with 256, 237 with 1024.
-// The generator and the smooth activations ask for more waves than that: 100000 x 2048 bf16 forward with dropout 292 us with 512
-// blocks, 185 with 1280; 100000 x 1024 fp32 184 with 256, 154 with 768.  Measured from 32 to 16384 features, 1000 to 2 M rows, fp32
+// The generator and the smooth activations ask for more waves than that: 100000 x 2048 bf16 forward with dropout 197 us with 1024
+// blocks, 187 with 1280; 100000 x 1024 fp32 169 with 256, 143 with 768.  Measured from 32 to 16384 features, 1000 to 2 M rows, fp32
 // and bf16, with and without dropout, in steps of 256 blocks: a CU more or less than the others counts (100000 x 1020 fp32 forward
 // 136 us with 256 blocks, 175 with 257).  Backward teams of 8 and 16 waves fit once on a CU.
 inline int64_t clamped(int64_t v, int64_t low, int64_t high) { return v < low ? low : v > high ? high : v; }
@@ -930,9 +932,12 @@ inline int64_t backward_blocks(const TailArgs& a, const Shape& h) {
   const int64_t least = a.drop && half && h.w < 8 ? 512 : 256;
   int64_t blocks = clamped(even((6 << 20) / (2 * block_bytes(a, h))), least, h.w < 8 ? 768 : 256);
   const int64_t sweeps = cdiv(a.rows, teams_in_block(h));
-  // A block's partial sums cost 8 bytes a feature each way, and its join some microseconds: at least 3 sweeps a block (6000 x 256 bf16
-  // 10.3 us with 256 blocks, 12.1 with 750; 2000 x 1021 13.0 and 16.7 with 500), 16 rows where a block takes one row at a time (5003 x
-  // 4096 bf16 33 us with 256, 35 with 512), 12 of one pack a lane (5003 x 1500 bf16 20.8 with 512, 24.7 with 256).
+  // A block's partial sums cost 8 bytes a feature each way, and its join some microseconds: at least 3 sweeps a block, and where a block
+  // takes one row at a time 12 rows of one pack a lane, 16 of more.  us with the rule, with that many rows, with that many:
+  //   3:  6000 x 256 bf16 10.6, with 1 12.3, with 12 10.7; 2000 x 1021 bf16 13.1, 16.2, 13.2; 20736 x 64 fp32 10.2, 10.5, 11.1;
+  //       30000 x 128 fp32 13.9, 14.1, 14.8
+  //   12: 5003 x 1500 bf16 20.5, with 3 21.1, with 24 24.7; 3000 x 2000 18.5, 21.2, 18.2; 10000 x 1200 24.8, 24.8, 27.7
+  //   16: 5003 x 4096 bf16 32.6, with 12 35.1, with 32 32.6; 8000 x 3000 36.3, 36.4, 42.5; 5003 x 2000 fp32 24.7, 25.6, 24.7
   blocks = clamped(even(sweeps / (h.w == 1 ? 3 : h.k == 1 ? 12 : 16)), 256, blocks);
   return sweeps <= 4 ? 1 : blocks_for(sweeps, blocks);  // a few rows: one block, no partial sums and no second launch
 }
