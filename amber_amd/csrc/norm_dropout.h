@@ -310,7 +310,8 @@ DEVINL void act_any(int act, float (&v)[N], float (&d)[N]) {
 // ---------------------------------------------------------------------------------------------------
 // without the norm: elementwise over the flat tensor, 16 bytes a thread, the next 16 on their way while these are worked on
 // (32768 x 4096 fp32 dropout 189 -> 177 us, 6.1 TB/s; 1.44 M x 128 fp32 with an activation 264 -> 245 forward, 446 -> 370 backward).
-// Bound by the memory; relu and leaky relu cost nothing beside it, gelu in fp32 2 % (248 us forward), in 16 bits more (1000003 x 333 fp16 with dropout 4.0 TB/s).
+// Bound by the memory; relu and leaky relu cost nothing beside it, gelu in fp32 2 % (248 us forward), in 16 bits
+// more (1000003 x 333 fp16 with dropout 4.0 TB/s).
 // ---------------------------------------------------------------------------------------------------
 template <class T, bool BWD, bool SMOOTH, int CACHE>
 __global__ __launch_bounds__(kBlock) void elementwise_kernel(TailArgs a) {
